@@ -301,6 +301,128 @@ VC4_API int vc4_logits_argmax_from(vc4_session* s, int slot, int src, int* token
 /* GPU::read_bytes (gpu.h:270) of a buffer, as floats (n values, q16 / 256). */
 VC4_API int vc4_read_buffer(vc4_session* s, int slot, int buf, int n, float* out);
 
+/* ---- Paged cache, chunk attention and draft verification ----------------------
+   No counterpart in the reference, which has one sequence and one contiguous
+   cache; these are vc4_attention_block's two halves (the K/V row appended, the
+   attention over the cached rows) for many sequences whose rows live in pages a
+   caller hands out, and the decision on drafted tokens that a verification pass
+   of the target model ends with.  All arrays are the caller's device buffers on
+   the GPU of `g`.  Nothing is allocated, freed or kept between calls: the work is
+   queued on `stream` (NULL: the stream of `g`) and the call returns without
+   waiting, so it may be captured into a CUDA graph (make one call of the same
+   shape before the capture, as with every kernel of this library).  Calls on
+   different streams may overlap when their outputs and work buffers are
+   distinct.  The caller's current device is left as it was.  A refused call
+   returns VC4_EINVAL and queues nothing.
+
+   What only the device knows (offsets, lengths, page ids, token ids, logits) is
+   checked by the kernels: a bad entry is skipped, never followed, and the largest
+   code seen is left in *status where the batch has one (set it to 0 before): a
+   page id outside the pool, a position outside the page table or the rotation
+   tables, a length below the new tokens, a token id outside the vocabulary give
+   VC4_EINVAL, a row of logits without a finite value VC4_ERANGE. */
+
+/* Element types of activations.  VC4_Q16I: int32 values on the q16 grid (1/256),
+   the form of this engine's own logits. */
+#define VC4_F32 0
+#define VC4_BF16 1
+#define VC4_F16 2
+#define VC4_Q16I 3
+
+/* Formats of cached values.  Q8 and Q16 are the slot cache's codec, byte for byte
+   (q8: int8 levels on the 1/16 grid; q16: big-endian int16 levels on the 1/2048
+   grid). */
+#define VC4_KV_Q8 8
+#define VC4_KV_Q16 16
+#define VC4_KV_BF16 1
+#define VC4_KV_F16 2
+
+/* A pool of pages: [pages][2: K, V][kv_heads][page_len][head_dim], packed, its
+   address a multiple of 16.  page_len: 16, 32, 64, 128 or 256; head_dim: a
+   multiple of 16, at most 128. */
+typedef struct {
+    void* data;
+    int format, pages, page_len, kv_heads, head_dim;
+} vc4_pages;
+
+/* Some new tokens of `seqs` sequences.  Row r of the activations is token
+   r - cu[s] of the sequence with cu[s] <= r < cu[s+1]; len[s] positions of
+   sequence s are in use, its new ones (the last cu[s+1] - cu[s]) among them;
+   position t lies in page table[s*table_stride + t/page_len] at t % page_len.  A
+   sequence may have no new token.  `tokens` bounds cu[seqs] (rows of it behind
+   the last sequence are left as they were), max_new and max_len bound the new
+   tokens and the length of one sequence: they choose the launch, so a captured
+   call holds for every content of the arrays within them. */
+typedef struct {
+    int seqs, tokens, max_new, max_len, table_stride;
+    const int* cu;       /* seqs + 1 */
+    const int* len;      /* seqs */
+    const int* table;    /* seqs x table_stride */
+    int* status;         /* one int, or NULL */
+} vc4_paged_batch;
+
+/* The append half of vc4_attention_block (gpu.h:142) over pages: each row of qkv
+   ([heads + 2*kv_heads][head_dim], rows qkv_stride elements apart; 0: packed) is
+   split; q and k heads are normalised (q_norm / k_norm: head_dim weights, both or
+   neither; 1/sqrt(mean square + eps), the squares summed in double) and rotated
+   by row `position` of cos / sin (rope_len x head_dim/2, both or neither; pairs
+   (i, i + head_dim/2) with rope_half, else (2i, 2i+1)); k and v are written into
+   the sequence's page, the rotated q to q ([heads][head_dim], q_stride apart).
+   The operations and their order are the slot cache's, so the page bytes of the
+   q8 / q16 formats are those vc4_kv_read_rows gives.  qkv_type and q_type:
+   VC4_F32, VC4_BF16 or VC4_F16.  Two sequences must not append into one page.
+   Addresses are multiples of 16, strides of 8 elements. */
+VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* qkv, int qkv_type,
+                             long long qkv_stride, int heads, const float* q_norm, const float* k_norm, float eps,
+                             const float* cos, const float* sin, int rope_len, int rope_half, void* q, int q_type,
+                             long long q_stride, void* stream);
+
+/* The attention half over pages: out = softmax(scale * q K^T) V, new token i of a
+   sequence seeing positions 0 .. len - new + i; query head h reads KV head
+   h / (heads / kv_heads).  scale 0: 1/sqrt(head_dim).  q_type is VC4_BF16 or
+   VC4_F16 and, for bf16 and f16 pages, the pages' own; out_type any of VC4_F32,
+   VC4_BF16, VC4_F16.  Products run on the tensor cores (bf16 pages: bf16, others:
+   f16; a bf16 q beyond +-65504 is taken as that), sums and softmax statistics in
+   float.  A row that sees no position is zero.  work: work_bytes of
+   vc4_paged_attention_bytes for the same pages, heads and batch bounds (NULL when
+   that is 0), free again when the call's work is done. */
+VC4_API int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* q, int q_type,
+                                long long q_stride, int heads, float scale, void* out, int out_type,
+                                long long out_stride, void* work, size_t work_bytes, void* stream);
+VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, int heads,
+                                      size_t* bytes);
+
+/* Which drafted tokens stand, and the token that follows them.  Sequence s fed the
+   target model rows cu[s] .. cu[s+1]-1: its last token, then its drafts; `fed`
+   holds those ids, `logits` (rows logits_stride elements apart; 0: vocab) what
+   each row predicts, p = softmax(logits / temperature) (temperature 0: the first
+   maximum).  The draft after row i of sequence s (the next fed id, x) is accepted
+   while u[row] * d(x) < p(x), d being the draft's row of draft_probs (one row for
+   each draft of the batch in order, probs_stride apart; 0: vocab), or one at x and
+   zero elsewhere when draft_probs is NULL.  The first refused row is sampled from max(p - d, 0) normalised (from p
+   where that is zero everywhere), and the last row, when all are accepted, from p:
+   the first id whose cumulative sum exceeds u_sample[s] times the total, sums in
+   double.  next: per row the accepted draft, then the sampled id, then -1;
+   accepted (seqs): drafts accepted; prob (rows, or NULL): the target's probability
+   of each id in next, 0 where that is -1.  logits_type: VC4_F32, VC4_BF16, VC4_F16
+   or VC4_Q16I.  `rows` bounds cu[seqs].  NaN logits count as -inf. */
+VC4_API int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const int* cu, const int* fed,
+                             const void* logits, int logits_type, long long logits_stride, const float* draft_probs,
+                             long long probs_stride, float temperature, const float* u, const float* u_sample,
+                             int* next, int* accepted, float* prob, int* status, void* work, size_t work_bytes,
+                             void* stream);
+VC4_API int vc4_verify_draft_bytes(int seqs, int rows, int vocab, size_t* bytes);
+
+/* One speculative decoding step of a slot: the last token and n-1 drafts, fed at
+   positions pos0 .. pos0+n-1 (the results of vc4_step position by position, in one
+   pass where the many-sequence kernels hold the model), then vc4_verify_draft on
+   the logits.  Host arrays: tokens (n), draft_probs ((n-1) x vocab, or NULL), u
+   (n-1); next (n) and prob (n, or NULL) as above, *accepted the drafts accepted:
+   positions pos0 .. pos0 + *accepted are decoded, the rows behind them are
+   overwritten by the next step.  n is at most the session's slots.  Synchronous. */
+VC4_API int vc4_step_draft(vc4_session* s, int slot, const int* tokens, int n, int pos0, const float* draft_probs,
+                           float temperature, const float* u, float u_sample, int* next, int* accepted, float* prob);
+
 /* draws()/syncs() (gpu.h:44-48): kernels launched and host syncs so far. */
 VC4_API int vc4_counters(const vc4_session* s, long long* launches, long long* syncs);
 /* Kernels one decode pass of n sequences launches. */

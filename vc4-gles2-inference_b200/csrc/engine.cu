@@ -78,6 +78,8 @@ struct vc4_session {
     cudaStream_t stream = nullptr;
     void* ops = nullptr;                      // buffers of the per-op calls (ops.cu), made on first use
     std::vector<int> plen;                    // host mirror of st.plen (shared-prefix rows per slot)
+    char* draft = nullptr;                    // device buffers of vc4_step_draft, made on first use
+    size_t draft_bytes = 0;
 };
 
 // ---------------------------------------------------------------------------
@@ -524,6 +526,7 @@ void vc4_session_destroy(vc4_session* s) {
     cudaStreamSynchronize(s->stream);
     free_op_buffers(s->ops);
     s->ops = nullptr;
+    if (s->draft) cudaFree(s->draft);
     for (auto& kv : s->graphs) cudaGraphExecDestroy(kv.second);
     s->graphs.clear();
     State& st = s->st;
@@ -707,6 +710,93 @@ int vc4_prefill_batch(vc4_session* s, int slot, const int* tokens, int n, int po
 int vc4_prefill_logits(vc4_session* s, int slot, const int* tokens, int n, int pos0, float* logits_all) {
     if (!logits_all) return fail(VC4_EINVAL, "logits_all is required");
     return prefill_batched(s, slot, tokens, n, pos0, nullptr, logits_all);
+}
+
+// One pass over the last token and its drafts, then the verification kernels on
+// the pass's own logits.  A batched prefill pass gives each position vc4_step's
+// logits bit for bit, so the drafts cost one pass; models and lengths outside
+// the many-sequence kernels step position by position into a logits buffer.
+int vc4_step_draft(vc4_session* s, int slot, const int* tokens, int n, int pos0, const float* draft_probs,
+                   float temperature, const float* u, float u_sample, int* next, int* accepted, float* prob) {
+    if (!s) return fail(VC4_EINVAL, "step_draft: session is null");
+    if (n <= 0 || n > s->slots) return fail(VC4_EINVAL, "step_draft: the fed tokens must be 1 .. slots");
+    if (!tokens || !next || !accepted || (n > 1 && !u)) return fail(VC4_EINVAL, "step_draft: a required array is null");
+    if (!(temperature >= 0.0f) || !(temperature < INFINITY))
+        return fail(VC4_EINVAL, "step_draft: temperature must not be negative");
+    if (int e = check_slot_pos(s, slot, pos0)) return e;
+    if (n > s->st.seq - pos0) return fail(VC4_EINVAL, "step_draft: the drafts run past the sequence length");
+    const DModel& m = s->m->d;
+    const int V = m.h.vocab;
+    for (int i = 0; i < n; ++i)
+        if (tokens[i] < 0 || tokens[i] >= V) return fail(VC4_EINVAL, "token id out of range");
+    CK(cudaSetDevice(m.device));
+    if (int e = session_unshare(s, slot, pos0)) return e;
+    size_t work = 0;
+    if (int e = vc4_verify_draft_bytes(1, n, V, &work)) return e;
+    // [cu 2 | fed n | u n | u_sample | next n | accepted | prob n | status] words, work, logits or draft rows
+    const bool batched = n > 1 && s->st.batch_ok && prefill_attention_fits(m, s->st);
+    const size_t words = ((size_t)(4 * n + 5) * 4 + 255) & ~(size_t)255, workb = (work + 255) & ~(size_t)255;
+    const size_t lgb = batched ? 0 : (size_t)n * V * 4, pb = draft_probs ? (size_t)(n - 1) * V * 4 : 0;
+    const size_t need = words + workb + lgb + pb;
+    if (need > s->draft_bytes) {
+        CK(cudaStreamSynchronize(s->stream));
+        if (s->draft) cudaFree(s->draft);
+        s->draft = nullptr;
+        s->draft_bytes = 0;
+        CK(cudaMalloc((void**)&s->draft, need));
+        s->draft_bytes = need;
+    }
+    int* d_cu = (int*)s->draft;
+    int* d_fed = d_cu + 2;
+    float* d_u = (float*)(d_fed + n);
+    float* d_us = d_u + n;
+    int* d_next = (int*)(d_us + 1);
+    int* d_acc = d_next + n;
+    float* d_prob = (float*)(d_acc + 1);
+    int* d_status = (int*)(d_prob + n);
+    void* d_work = s->draft + words;
+    int32_t* d_lg = (int32_t*)(s->draft + words + workb);
+    float* d_dp = (float*)(s->draft + words + workb + lgb);
+
+    const int32_t* logits = d_lg;
+    if (batched) {
+        int* hp = s->h_pin;
+        for (int i = 0; i < n; ++i) { hp[i] = slot; hp[n + i] = tokens[i]; hp[2 * n + i] = pos0 + i; }
+        int* dcall = s->d_slot;
+        CK(cudaMemcpyAsync(dcall, hp, sizeof(int) * 3 * n, cudaMemcpyHostToDevice, s->stream));
+        PassArgs a{n, dcall, dcall + n, dcall + 2 * n, s->d_next, 0, nullptr, 1};
+        if (int e = run_pass(s, a)) return e;
+        logits = s->st.logits;
+    } else {
+        for (int i = 0; i < n; ++i) {
+            const int p = pos0 + i;
+            if (int e = host_step(s, 1, &slot, tokens + i, &p, nullptr, nullptr)) return e;
+            CK(cudaMemcpyAsync(d_lg + (size_t)i * V, s->st.logits, sizeof(int32_t) * V, cudaMemcpyDeviceToDevice, s->stream));
+        }
+    }
+    std::vector<int> in(2 * n + 3);
+    in[0] = 0;
+    in[1] = n;
+    memcpy(&in[2], tokens, sizeof(int) * n);
+    if (n > 1) memcpy(&in[2 + n], u, sizeof(float) * (n - 1));
+    memcpy(&in[2 + 2 * n], &u_sample, sizeof(float));
+    CK(cudaMemcpyAsync(s->draft, in.data(), sizeof(int) * in.size(), cudaMemcpyHostToDevice, s->stream));
+    CK(cudaMemsetAsync(d_status, 0, sizeof(int), s->stream));
+    if (pb) CK(cudaMemcpyAsync(d_dp, draft_probs, pb, cudaMemcpyHostToDevice, s->stream));
+    if (int e = vc4_verify_draft(s->m->g, 1, n, V, d_cu, d_fed, logits, VC4_Q16I, V, pb ? d_dp : nullptr, V, temperature,
+                                 d_u, d_us, d_next, d_acc, d_prob, d_status, d_work, work, s->stream))
+        return e;
+    s->launches += 2;
+    std::vector<int> out(2 * n + 2);   // next, accepted, prob, status
+    CK(cudaMemcpyAsync(out.data(), d_next, sizeof(int) * out.size(), cudaMemcpyDeviceToHost, s->stream));
+    CK(cudaStreamSynchronize(s->stream));
+    s->syncs++;
+    if (int e = check_kernel_word(s)) return e;
+    if (out[2 * n + 1]) return fail(out[2 * n + 1], "step_draft: the verification kernels' self-check failed");
+    memcpy(next, out.data(), sizeof(int) * n);
+    *accepted = out[n];
+    if (prob) memcpy(prob, &out[n + 1], sizeof(float) * n);
+    return VC4_OK;
 }
 
 int vc4_kv_row_bytes(const vc4_session* s) { return s->st.row_bytes; }
@@ -1129,6 +1219,10 @@ namespace vc4 {
 int set_error(int code, const char* msg) { return fail(code, msg); }
 
 const DModel& model_of(const vc4_model* m) { return m->d; }
+
+int gpu_device(const vc4_gpu* g) { return g->device; }
+
+cudaStream_t gpu_stream(const vc4_gpu* g) { return g->stream; }
 
 SessionView session_view(vc4_session* s) {
     SessionView v;

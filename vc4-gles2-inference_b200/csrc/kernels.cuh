@@ -1488,6 +1488,31 @@ __global__ void __launch_bounds__(kThreads) k_logits_wide(DMat W, const float* r
     logits_finish(s, b0, nb, fz);
 }
 
+// The packed bytes of one value (the inverse of kv_word), as the low bits of a word.
+__device__ __forceinline__ unsigned kv_encode(float x, int kvb, float* dec) {
+    if (kvb == 2) {
+        float q = floorf(__fadd_rn(__fmul_rn(x, 2048.0f), 0.5f));
+        q = q < -32768.0f ? -32768.0f : q > 32767.0f ? 32767.0f : q;
+        *dec = __fmul_rn(q, 1.0f / 2048.0f);
+        const unsigned u = (unsigned)(int)q & 0xFFFFu;
+        return (u >> 8) | ((u & 0xFFu) << 8);           // big-endian byte order in memory
+    }
+    float q = floorf(__fadd_rn(__fmul_rn(x, 16.0f), 0.5f));
+    q = q < -128.0f ? -128.0f : q > 127.0f ? 127.0f : q;
+    *dec = __fmul_rn(q, 1.0f / 16.0f);
+    return (unsigned)(int)q & 0xFFu;
+}
+
+// ldmatrix of four 8x8 16-bit matrices (row addresses from lanes 0-7, 8-15,
+// 16-23, 24-31), plain and transposed.
+__device__ __forceinline__ void ldsm_x4(unsigned addr, unsigned (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(unsigned addr, unsigned (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
 #ifdef VC4_COMMON_TU
 // Attention for one (KV head, sequence) runs on group/hq clusters of kAttnCtas
 // CTAs, each cluster serving hq of the KV head's query heads, with a single
@@ -1605,21 +1630,6 @@ __device__ __forceinline__ int kv_codes(unsigned w, int kvb, float* out) {
     for (int j = 0; j < 4; ++j) out[j] = (float)(signed char)((w >> (8 * j)) & 0xFFu);
     return 4;
 }
-// The packed bytes of one value (the inverse of kv_word), as the low bits of a word.
-__device__ __forceinline__ unsigned kv_encode(float x, int kvb, float* dec) {
-    if (kvb == 2) {
-        float q = floorf(__fadd_rn(__fmul_rn(x, 2048.0f), 0.5f));
-        q = q < -32768.0f ? -32768.0f : q > 32767.0f ? 32767.0f : q;
-        *dec = __fmul_rn(q, 1.0f / 2048.0f);
-        const unsigned u = (unsigned)(int)q & 0xFFFFu;
-        return (u >> 8) | ((u & 0xFFu) << 8);           // big-endian byte order in memory
-    }
-    float q = floorf(__fadd_rn(__fmul_rn(x, 16.0f), 0.5f));
-    q = q < -128.0f ? -128.0f : q > 127.0f ? 127.0f : q;
-    *dec = __fmul_rn(q, 1.0f / 16.0f);
-    return (unsigned)(int)q & 0xFFu;
-}
-
 // Attention weights of hq heads over positions 0..len-1 (sc[hh*seq + t]), in
 // place: kWarps / hq warps per head (one when there are more heads than
 // warps) take the maximum, then E_t = rint(exp(s_t - max) * 2^k), an integer
@@ -1997,16 +2007,6 @@ __host__ __device__ inline size_t attnb_smem_bytes(int hq, int hd, int seq, int 
     return attnb_carve(hq, hd, seq, kv_bits, nullptr, nullptr);
 }
 
-// ldmatrix of four 8x8 16-bit matrices (row addresses from lanes 0-7, 8-15,
-// 16-23, 24-31), plain and transposed.
-__device__ __forceinline__ void ldsm_x4(unsigned addr, unsigned (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(unsigned addr, unsigned (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
 // D += A (16x32, 8-bit, row) * B (32x8, 8-bit, col), int32 accumulators;
 // AU / BU select unsigned operands.
 template <bool AU, bool BU>

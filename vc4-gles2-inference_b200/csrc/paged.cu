@@ -1,0 +1,463 @@
+// paged.cu -- the paged KV cache: the append kernel (QK-norm, RoPE and the cache
+// codec over a projection's rows), the join of split attention, and the C entries.
+#include "paged.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+namespace vc4 {
+namespace {
+
+int fail(int code, const std::string& msg) { return set_error(code, msg.c_str()); }
+
+// The GPU of a handle as the current device for one call; the caller's after it.
+struct OnDevice {
+    int before = -1;
+    cudaError_t err;
+    explicit OnDevice(int device) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+        else if (err == cudaSuccess) before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+
+struct AppendArgs {
+    PagedArgs p;
+    const void* qkv;
+    void* q;
+    long long qkv_stride, q_stride;
+    const float *q_norm, *k_norm, *cos, *sin;
+    float eps;
+    int heads, rope_len, half, q_type, per_block;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendTokens = 8;    // most tokens of a block (one warp looks one up)
+
+// Four consecutive values of a row as floats.
+template <int TIN>
+__device__ __forceinline__ float4 load4(const void* row, long long i) {
+    if (TIN == VC4_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + i);
+    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(row) + i);
+    if (TIN == VC4_BF16)
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
+                           __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// Four consecutive values of a cached row, in the pages' format.
+template <int FMT>
+__device__ __forceinline__ void store_cache4(uint8_t* row, int i, float4 v) {
+    float dec;
+    if (FMT == P_Q8) {
+        *reinterpret_cast<unsigned*>(row + i) = kv_encode(v.x, 1, &dec) | kv_encode(v.y, 1, &dec) << 8 |
+                                                kv_encode(v.z, 1, &dec) << 16 | kv_encode(v.w, 1, &dec) << 24;
+    } else if (FMT == P_Q16) {
+        *reinterpret_cast<uint2*>(row + 2 * i) = make_uint2(kv_encode(v.x, 2, &dec) | kv_encode(v.y, 2, &dec) << 16,
+                                                            kv_encode(v.z, 2, &dec) | kv_encode(v.w, 2, &dec) << 16);
+    } else {
+        constexpr int F = FMT == P_BF16 ? P_BF16 : P_F16;
+        *reinterpret_cast<uint2*>(row + 2 * i) = make_uint2(pack_op<F>(v.x, v.y), pack_op<F>(v.z, v.w));
+    }
+}
+
+// One group of LPV lanes per head vector (hd/8 of them at work): a lane holds
+// eight values as four rotation pairs, so norm, rotation and encoding stay in
+// its registers and every load and store is 4 to 16 bytes wide.  Bound by bytes
+// for many tokens, by the chain offsets -> length -> page id for a few; the first
+// vector's loads are issued before that chain.  The float operations are the slot
+// cache's (k_attn): squares summed in double, 1/sqrt(ss/hd + eps), w*(r*x), the
+// rotation's products and sums rounded one by one, the codec's floor(x*grid + 1/2).
+template <int TIN, int FMT>
+__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
+    const PagedArgs& p = a.p;
+    const int hd = p.head_dim, half = hd / 2, nvec = a.heads + 2 * p.kv_heads;
+    __shared__ int s_pos[kAppendTokens];             // the position, -1: nothing to do
+    __shared__ long long s_row[kAppendTokens];       // row index of (page, K, head 0, offset)
+    const int lpv = hd > 64 ? 16 : hd > 32 ? 8 : hd > 16 ? 4 : 2;
+    const int tok0 = blockIdx.x * a.per_block, ntok = min(a.per_block, p.tokens - tok0);
+    const int sub = threadIdx.x % lpv, grp = threadIdx.x / lpv, ngrp = kAppendThreads / lpv;
+    const bool live = sub * 8 < hd;
+    const int i0 = a.half ? 4 * sub : 8 * sub, i1 = a.half ? half + 4 * sub : 8 * sub + 4;
+    const int total = ntok * nvec;
+    auto fetch = [&](int it, float4& x0, float4& x1) {
+        if (it < total && live) {
+            const long long base = (long long)(tok0 + it / nvec) * a.qkv_stride + (long long)(it % nvec) * hd;
+            x0 = load4<TIN>(a.qkv, base + i0);
+            x1 = load4<TIN>(a.qkv, base + i1);
+        }
+    };
+    float4 x0 = make_float4(0, 0, 0, 0), x1 = x0;
+    fetch(grp, x0, x1);
+
+    const int warp = threadIdx.x >> 5;
+    if (warp < ntok) {
+        const int tok = tok0 + warp, s = paged_find(p.cu, p.seqs, tok);
+        const int c0 = p.cu[s], c1 = p.cu[s + 1];
+        int pos = -1;
+        long long row = 0;
+        if (tok >= c0 && tok < c1) {                 // rows behind the last sequence: none of this
+            const int page_len = 1 << p.page_shift;
+            pos = p.len[s] - (c1 - tok);
+            bool bad = pos < 0 || pos >= (long long)p.table_stride * page_len || (a.cos && pos >= a.rope_len) ||
+                       c1 - c0 > p.max_new;
+            if (!bad) {
+                const int page = p.table[(size_t)s * p.table_stride + (pos >> p.page_shift)];
+                bad = page < 0 || page >= p.pages;
+                row = (((long long)page * 2 * p.kv_heads) << p.page_shift) + (pos & (page_len - 1));
+            }
+            if (bad) {
+                if ((threadIdx.x & 31) == 0) paged_flag(p.status, VC4_EINVAL);
+                pos = -1;
+            }
+        }
+        if ((threadIdx.x & 31) == 0) {
+            s_pos[warp] = pos;
+            s_row[warp] = row;
+        }
+    }
+    __syncthreads();
+
+    const int es = FMT == P_Q8 ? 1 : 2;
+    // every lane of a warp runs the same number of rounds (the sums shuffle)
+    for (int it0 = 0; it0 < total; it0 += ngrp) {
+        const int it = it0 + grp;
+        float4 n0 = make_float4(0, 0, 0, 0), n1 = n0;
+        fetch(it + ngrp, n0, n1);
+        const int t = min(it, total - 1) / nvec, vec = min(it, total - 1) % nvec;
+        const int pos = it < total ? s_pos[t] : -1;
+        if (a.q_norm) {
+            double acc = 0.0;
+            acc = fma((double)x0.x, (double)x0.x, acc);   // a product of two floats is exact in double
+            acc = fma((double)x0.y, (double)x0.y, acc);
+            acc = fma((double)x0.z, (double)x0.z, acc);
+            acc = fma((double)x0.w, (double)x0.w, acc);
+            acc = fma((double)x1.x, (double)x1.x, acc);
+            acc = fma((double)x1.y, (double)x1.y, acc);
+            acc = fma((double)x1.z, (double)x1.z, acc);
+            acc = fma((double)x1.w, (double)x1.w, acc);
+            if (!live) acc = 0.0;
+            for (int o = lpv / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+            if (vec < a.heads + p.kv_heads && live) {
+                const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(__double2float_rn(acc), (float)hd), a.eps)));
+                const float* w = vec < a.heads ? a.q_norm : a.k_norm;
+                const float4 w0 = *reinterpret_cast<const float4*>(w + i0), w1 = *reinterpret_cast<const float4*>(w + i1);
+                x0 = make_float4(__fmul_rn(w0.x, __fmul_rn(r, x0.x)), __fmul_rn(w0.y, __fmul_rn(r, x0.y)),
+                                 __fmul_rn(w0.z, __fmul_rn(r, x0.z)), __fmul_rn(w0.w, __fmul_rn(r, x0.w)));
+                x1 = make_float4(__fmul_rn(w1.x, __fmul_rn(r, x1.x)), __fmul_rn(w1.y, __fmul_rn(r, x1.y)),
+                                 __fmul_rn(w1.z, __fmul_rn(r, x1.z)), __fmul_rn(w1.w, __fmul_rn(r, x1.w)));
+            }
+        }
+        if (pos >= 0 && live) {
+            if (a.cos && vec < a.heads + p.kv_heads) {
+                const float4 c = *reinterpret_cast<const float4*>(a.cos + (size_t)pos * half + 4 * sub);
+                const float4 s = *reinterpret_cast<const float4*>(a.sin + (size_t)pos * half + 4 * sub);
+                auto turn = [](float& u, float& v, float cc, float ss) {
+                    const float y = __fsub_rn(__fmul_rn(u, cc), __fmul_rn(v, ss));
+                    v = __fadd_rn(__fmul_rn(u, ss), __fmul_rn(v, cc));
+                    u = y;
+                };
+                if (a.half) {
+                    turn(x0.x, x1.x, c.x, s.x);
+                    turn(x0.y, x1.y, c.y, s.y);
+                    turn(x0.z, x1.z, c.z, s.z);
+                    turn(x0.w, x1.w, c.w, s.w);
+                } else {
+                    turn(x0.x, x0.y, c.x, s.x);
+                    turn(x0.z, x0.w, c.y, s.y);
+                    turn(x1.x, x1.y, c.z, s.z);
+                    turn(x1.z, x1.w, c.w, s.w);
+                }
+            }
+            if (vec < a.heads) {
+                const long long at = (long long)(tok0 + t) * a.q_stride + (long long)vec * hd;
+                store4_as(a.q, a.q_type, at + i0, x0);
+                store4_as(a.q, a.q_type, at + i1, x1);
+            } else {
+                // heads of K, then of V, lie page_len rows apart
+                uint8_t* row = p.data + (s_row[t] + ((long long)(vec - a.heads) << p.page_shift)) * (hd * es);
+                store_cache4<FMT>(row, i0, x0);
+                store_cache4<FMT>(row, i1, x1);
+            }
+        }
+        x0 = n0;
+        x1 = n1;
+    }
+}
+
+template <int FMT>
+void launch_append(const AppendArgs& a, int type, unsigned blocks, cudaStream_t st) {
+    if (type == VC4_F32) k_paged_append<VC4_F32, FMT><<<blocks, kAppendThreads, 0, st>>>(a);
+    else if (type == VC4_BF16) k_paged_append<VC4_BF16, FMT><<<blocks, kAppendThreads, 0, st>>>(a);
+    else k_paged_append<VC4_F16, FMT><<<blocks, kAppendThreads, 0, st>>>(a);
+}
+
+// ---------------------------------------------------------------------------
+// join of split attention: o = sum_i 2^(c(m_i - m)) O_i / sum_i 2^(c(m_i - m)) l_i
+// ---------------------------------------------------------------------------
+
+// One warp per (token, head); lane i holds the weights of splits i and i + 32.
+__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a) {
+    pdl_wait();
+    const int tok = blockIdx.x, lane = threadIdx.x & 31;
+    const PagedArgs& p = a.p;
+    const int last = min(p.cu[p.seqs], p.tokens);
+    if (tok >= last) return;
+    // rows of a sequence beyond max_new were not computed: leave them
+    const int s = paged_find(p.cu, p.seqs, tok);
+    if (tok < p.cu[s] || tok >= p.cu[s + 1] || tok - p.cu[s] >= p.max_new) return;
+    const int hd = p.head_dim;
+    for (int head = threadIdx.x >> 5; head < a.heads; head += blockDim.x >> 5) {
+        const size_t at = (size_t)tok * a.heads + head, step = (size_t)p.tokens * a.heads;
+        float2 e[2];
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            e[k] = lane + 32 * k < a.splits ? a.ml[at + (lane + 32 * k) * step] : make_float2(-INFINITY, 0.0f);
+            m = fmaxf(m, e[k].x);
+        }
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float w[2], l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            w[k] = e[k].x == -INFINITY ? 0.0f : ex2f((e[k].x - m) * a.scale2);
+            if (w[k] != 0.0f) l = __fmaf_rn(w[k], e[k].y, l);
+        }
+        // NaN statistics (a NaN score) have m_i = -inf or a NaN sum: the sum carries them
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (e[k].y != e[k].y) l = e[k].y;
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float f = l > 0.0f || l != l ? a.vscale / l : 0.0f;
+        for (int d0 = 0; d0 < hd; d0 += 128) {
+            const int d = d0 + 4 * lane;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int i = 0; i < a.splits; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, i < 32 ? w[0] : w[1], i & 31);
+                if (wi == 0.0f || d >= hd) continue;     // an empty split left nothing to read
+                const float4 x = *reinterpret_cast<const float4*>(a.part + (at + i * step) * hd + d);
+                v.x = __fmaf_rn(wi, x.x, v.x);
+                v.y = __fmaf_rn(wi, x.y, v.y);
+                v.z = __fmaf_rn(wi, x.z, v.z);
+                v.w = __fmaf_rn(wi, x.w, v.w);
+            }
+            if (d < hd)
+                store4_as(a.out, a.out_type, (long long)tok * a.out_stride + (long long)head * hd + d,
+                          make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// argument checks and plans
+// ---------------------------------------------------------------------------
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+std::string bad_pages(const vc4_pages* p) {
+    if (!p) return "pages is null";
+    if (p->format != VC4_KV_Q8 && p->format != VC4_KV_Q16 && p->format != VC4_KV_BF16 && p->format != VC4_KV_F16)
+        return "unknown page format " + std::to_string(p->format);
+    if (p->page_len != 16 && p->page_len != 32 && p->page_len != 64 && p->page_len != 128 && p->page_len != 256)
+        return "page_len must be 16, 32, 64, 128 or 256";
+    if (p->pages <= 0 || p->kv_heads <= 0) return "pages and kv_heads must be positive";
+    if (p->head_dim <= 0 || p->head_dim > 128 || p->head_dim % 16) return "head_dim must be a multiple of 16, at most 128";
+    if (!p->data || !aligned16(p->data)) return "the pool's address must be a multiple of 16";
+    return "";
+}
+
+std::string bad_batch(const vc4_paged_batch* b, const vc4_pages* p) {
+    if (!b) return "batch is null";
+    if (b->seqs <= 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_stride <= 0)
+        return "seqs and table_stride must be positive, tokens, max_new and max_len not negative";
+    if (!b->cu || !b->len || !b->table) return "cu, len and table are required";
+    if ((long long)b->max_len > (long long)b->table_stride * p->page_len) return "max_len runs past the page table";
+    return "";
+}
+
+std::string bad_rows(const char* what, const void* ptr, long long stride, long long width) {
+    if (!ptr || !aligned16(ptr)) return std::string(what) + "'s address must be a multiple of 16";
+    if (stride < width || stride % 8) return std::string(what) + "'s stride must be a multiple of 8 elements, at least a row";
+    return "";
+}
+
+int shift_of(int page_len) { return page_len == 16 ? 4 : page_len == 32 ? 5 : page_len == 64 ? 6 : page_len == 128 ? 7 : 8; }
+
+PagedArgs paged_args(const vc4_pages* p, const vc4_paged_batch* b) {
+    PagedArgs a{};
+    a.data = (uint8_t*)p->data;
+    a.pages = p->pages; a.page_shift = shift_of(p->page_len); a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
+    a.seqs = b->seqs; a.tokens = b->tokens; a.max_new = b->max_new; a.table_stride = b->table_stride;
+    a.cu = b->cu; a.len = b->len; a.table = b->table; a.status = b->status;
+    return a;
+}
+
+int pfmt(int format) {
+    return format == VC4_KV_Q8 ? P_Q8 : format == VC4_KV_Q16 ? P_Q16 : format == VC4_KV_BF16 ? P_BF16 : P_F16;
+}
+
+struct AttnPlan {
+    int wr, row_tiles, splits;
+    size_t bytes;
+};
+
+// Rows of a block: the least of 16, 32 and 64 that holds one sequence's rows.
+// Splits: enough blocks for two on each of the GPU's SMs, but at least two tiles
+// of 64 positions each (a split costs a partial result and a second kernel).
+AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms) {
+    AttnPlan pl{};
+    const long long rows = (long long)b->max_new * (heads / p->kv_heads);
+    pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    pl.row_tiles = (int)((rows + 16 * pl.wr - 1) / (16 * pl.wr));
+    const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
+    const int tiles = (b->max_len + kPagedTile - 1) / kPagedTile;
+    const long long want = (2 * (long long)sms + units - 1) / units;
+    pl.splits = (int)std::max(1LL, std::min({want, (long long)tiles / 2, (long long)kPagedMaxSplits}));
+    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
+    return pl;
+}
+
+int sms_of(int device, int* sms) {
+    static int have[64] = {};
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lk(mu);
+    if (device < 0 || device >= 64) return fail(VC4_EINVAL, "device index too large");
+    if (!have[device]) {
+        const cudaError_t e = cudaDeviceGetAttribute(&have[device], cudaDevAttrMultiProcessorCount, device);
+        if (e != cudaSuccess) return fail(VC4_ECUDA, cudaGetErrorString(e));
+    }
+    *sms = have[device];
+    return VC4_OK;
+}
+
+}  // namespace
+}  // namespace vc4
+
+using namespace vc4;
+
+extern "C" int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* qkv, int qkv_type,
+                                long long qkv_stride, int heads, const float* q_norm, const float* k_norm, float eps,
+                                const float* cos, const float* sin, int rope_len, int rope_half, void* q, int q_type,
+                                long long q_stride, void* stream) {
+    auto refuse = [](const std::string& m) { return fail(VC4_EINVAL, "paged_append: " + m); };
+    std::string m = bad_pages(p);
+    if (m.empty()) m = bad_batch(b, p);
+    if (!m.empty()) return refuse(m);
+    if (heads <= 0 || heads % p->kv_heads) return refuse("heads must be a positive multiple of kv_heads");
+    if (qkv_type < VC4_F32 || qkv_type > VC4_F16 || q_type < VC4_F32 || q_type > VC4_F16)
+        return refuse("qkv and q are VC4_F32, VC4_BF16 or VC4_F16");
+    const long long width = ((long long)heads + 2 * p->kv_heads) * p->head_dim, qw = (long long)heads * p->head_dim;
+    if (!qkv_stride) qkv_stride = width;
+    if (!q_stride) q_stride = qw;
+    m = bad_rows("qkv", qkv, qkv_stride, width);
+    if (m.empty()) m = bad_rows("q", q, q_stride, qw);
+    if (!m.empty()) return refuse(m);
+    if (!q_norm != !k_norm) return refuse("q_norm and k_norm go together");
+    if (q_norm && (!aligned16(q_norm) || !aligned16(k_norm))) return refuse("the norm weights' addresses must be multiples of 16");
+    if (q_norm && !(eps >= 0.0f)) return refuse("eps must not be negative");
+    if (!cos != !sin) return refuse("cos and sin go together");
+    if (cos && (!aligned16(cos) || !aligned16(sin) || rope_len <= 0))
+        return refuse("the rotation tables need rows, their addresses multiples of 16");
+    if (!g) return refuse("gpu is null");
+    if (!b->tokens || !b->max_new) return VC4_OK;
+    OnDevice on(gpu_device(g));
+    if (on.err != cudaSuccess) return fail(VC4_ECUDA, cudaGetErrorString(on.err));
+    cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : gpu_stream(g);
+    AppendArgs a{};
+    a.p = paged_args(p, b);
+    a.qkv = qkv; a.q = q; a.qkv_stride = qkv_stride; a.q_stride = q_stride;
+    a.q_norm = q_norm; a.k_norm = k_norm; a.cos = cos; a.sin = sin; a.eps = eps;
+    a.heads = heads; a.rope_len = rope_len; a.half = rope_half ? 1 : 0; a.q_type = q_type;
+    // one token per block while the blocks fit the GPU at once, then more, so
+    // that a block's look-up is shared by several rounds of vectors
+    a.per_block = b->tokens <= 1024 ? 1 : b->tokens <= 4096 ? 2 : 4;
+    const unsigned blocks = (unsigned)(((long long)b->tokens + a.per_block - 1) / a.per_block);
+    switch (pfmt(p->format)) {
+        case P_Q8: launch_append<P_Q8>(a, qkv_type, blocks, st); break;
+        case P_Q16: launch_append<P_Q16>(a, qkv_type, blocks, st); break;
+        case P_BF16: launch_append<P_BF16>(a, qkv_type, blocks, st); break;
+        default: launch_append<P_F16>(a, qkv_type, blocks, st); break;
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(VC4_ECUDA, std::string("paged_append: ") + cudaGetErrorString(e));
+    return VC4_OK;
+}
+
+extern "C" int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, int heads,
+                                         size_t* bytes) {
+    auto refuse = [](const std::string& m) { return fail(VC4_EINVAL, "paged_attention_bytes: " + m); };
+    std::string m = bad_pages(p);
+    if (m.empty()) m = bad_batch(b, p);
+    if (!m.empty()) return refuse(m);
+    if (heads <= 0 || heads % p->kv_heads) return refuse("heads must be a positive multiple of kv_heads");
+    if (!bytes) return refuse("bytes is null");
+    if (!g) return refuse("gpu is null");
+    int sms = 0;
+    if (int e = sms_of(gpu_device(g), &sms)) return e;
+    *bytes = attn_plan(p, b, heads, sms).bytes;
+    return VC4_OK;
+}
+
+extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* q, int q_type,
+                                   long long q_stride, int heads, float scale, void* out, int out_type,
+                                   long long out_stride, void* work, size_t work_bytes, void* stream) {
+    auto refuse = [](const std::string& m) { return fail(VC4_EINVAL, "paged_attention: " + m); };
+    std::string m = bad_pages(p);
+    if (m.empty()) m = bad_batch(b, p);
+    if (!m.empty()) return refuse(m);
+    if (heads <= 0 || heads % p->kv_heads) return refuse("heads must be a positive multiple of kv_heads");
+    if (q_type != VC4_BF16 && q_type != VC4_F16) return refuse("q is VC4_BF16 or VC4_F16");
+    if ((p->format == VC4_KV_BF16 && q_type != VC4_BF16) || (p->format == VC4_KV_F16 && q_type != VC4_F16))
+        return refuse("q has the pages' type where that is bf16 or f16");
+    if (out_type < VC4_F32 || out_type > VC4_F16) return refuse("out is VC4_F32, VC4_BF16 or VC4_F16");
+    const long long width = (long long)heads * p->head_dim;
+    if (!q_stride) q_stride = width;
+    if (!out_stride) out_stride = width;
+    m = bad_rows("q", q, q_stride, width);
+    if (m.empty()) m = bad_rows("out", out, out_stride, width);
+    if (!m.empty()) return refuse(m);
+    if (!(scale >= 0.0f) || !(scale < INFINITY)) return refuse("scale must not be negative (0: 1/sqrt(head_dim))");
+    if (!g) return refuse("gpu is null");
+    int sms = 0;
+    if (int e = sms_of(gpu_device(g), &sms)) return e;
+    const AttnPlan pl = attn_plan(p, b, heads, sms);
+    if (work_bytes < pl.bytes || (pl.bytes && (!work || !aligned16(work))))
+        return refuse("the work buffer needs " + std::to_string(pl.bytes) + " bytes at a multiple of 16");
+    if (!b->tokens || !b->max_new) return VC4_OK;
+    if ((long long)b->seqs * p->kv_heads * pl.row_tiles * pl.splits > 0x7fffffffLL) return refuse("too many rows in one call");
+    OnDevice on(gpu_device(g));
+    if (on.err != cudaSuccess) return fail(VC4_ECUDA, cudaGetErrorString(on.err));
+    cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : gpu_stream(g);
+    PagedAttnArgs a{};
+    a.p = paged_args(p, b);
+    a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.q_type = q_type; a.out_type = out_type;
+    a.heads = heads; a.group = heads / p->kv_heads; a.row_tiles = pl.row_tiles; a.splits = pl.splits;
+    const double grid = p->format == VC4_KV_Q8 ? 1.0 / 16 : p->format == VC4_KV_Q16 ? 1.0 / 2048 : 1.0;
+    const double sc = scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)p->head_dim);
+    a.scale2 = (float)(sc * 1.4426950408889634 * grid);
+    a.vscale = (float)grid;
+    if (pl.splits > 1) {
+        a.part = (float*)work;
+        a.ml = (float2*)((char*)work + (size_t)pl.splits * b->tokens * heads * p->head_dim * 4);
+    }
+    switch (pfmt(p->format)) {
+        case P_Q8: launch_paged_split_q8(a, pl.wr, st); break;
+        case P_Q16: launch_paged_split_q16(a, pl.wr, st); break;
+        case P_BF16: launch_paged_split_bf16(a, pl.wr, st); break;
+        default: launch_paged_split_f16(a, pl.wr, st); break;
+    }
+    if (pl.splits > 1) launch_pdl_block(k_paged_join, dim3((unsigned)b->tokens), 128, 0, st, a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(VC4_ECUDA, std::string("paged_attention: ") + cudaGetErrorString(e));
+    return VC4_OK;
+}

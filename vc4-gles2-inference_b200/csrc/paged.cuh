@@ -1,0 +1,161 @@
+// paged.cuh -- what the paged-cache kernels share: the launch arguments, where a
+// row of a sequence lies, the cached formats as tensor-core operands.
+//
+// A pool is [page][K, V][kv head][page_len][head_dim] values, so the rows of one
+// head inside a page are one contiguous piece, whatever the format.
+#pragma once
+#include "kernels.cuh"
+#include "../../include/vc4b200.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace vc4 {
+
+// Formats as template arguments.
+enum PFmt : int { P_Q8 = 0, P_Q16 = 1, P_BF16 = 2, P_F16 = 3 };
+
+// The pool and the batch, as every paged kernel gets them.
+struct PagedArgs {
+    uint8_t* data;
+    int pages, page_shift, kv_heads, head_dim;
+    int seqs, tokens, max_new, table_stride;
+    const int *cu, *len, *table;
+    int* status;
+};
+
+struct PagedAttnArgs {
+    PagedArgs p;
+    const void* q;
+    void* out;
+    long long q_stride, out_stride;
+    int q_type, out_type, heads, group;
+    int row_tiles, splits;   // grid: ((sequence * kv_heads + head) * row_tiles + tile) * splits + split
+    float scale2;            // score scale x log2 e x the K grid
+    float vscale;            // the V grid
+    float* part;             // [splits][tokens*heads][head_dim] unnormalised sums
+    float2* ml;              // [splits][tokens*heads] running maximum (of the unscaled score) and sum
+};
+
+// The split kernels of one format (paged_*.cu); wr: 16-row tiles per block (1, 2 or 4).
+void launch_paged_split_q8(const PagedAttnArgs& a, int wr, cudaStream_t st);
+void launch_paged_split_q16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+void launch_paged_split_bf16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+void launch_paged_split_f16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+
+namespace {
+
+constexpr int kPagedSplitThreads = 128;
+constexpr int kPagedTile = 64;      // positions per K/V tile of the split kernels
+constexpr int kPagedMaxSplits = 64;
+
+__device__ __forceinline__ void paged_flag(int* status, int code) {
+    if (status) atomicMax(status, code);
+}
+
+// The sequence that holds row `r`: the last s with cu[s] <= r, by a 32-way
+// search of one warp (every lane returns it).  Any contents of cu give an s in
+// [0, seqs).
+__device__ __forceinline__ int paged_find(const int* cu, int seqs, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = seqs;
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lo + lane * step;
+        const bool le = lane * step < n && cu[at] <= r;
+        // the candidates are ordered: the last lane that holds
+        const unsigned m = __ballot_sync(0xffffffffu, le);
+        const int last = m ? 31 - __clz(m) : 0;
+        n = min(step, n - last * step);
+        lo += last * step;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int FMT> struct PagedBytes { static constexpr int v = FMT == P_Q8 ? 1 : 2; };
+
+// Two 16-bit operands in one register.
+__device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    unsigned r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <int FMT>
+__device__ __forceinline__ unsigned pack_op(float lo, float hi) {
+    return FMT == P_BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+}
+// Two bf16 query values as f16: exact inside f16's normal range (8 significant
+// bits go into 11); beyond +-65504 the largest f16, and below 2^-14 the error is
+// at most 2^-25 absolute.  NaN stays NaN.
+__device__ __forceinline__ unsigned bf16_to_f16(unsigned w) {
+    float lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+    lo = lo > 65504.0f ? 65504.0f : lo < -65504.0f ? -65504.0f : lo;
+    hi = hi > 65504.0f ? 65504.0f : hi < -65504.0f ? -65504.0f : hi;
+    return pack_f16(lo, hi);
+}
+// Two q16 levels (big-endian int16 in memory) as f16: 2^23 + (level + 2^15)
+// built in the mantissa, so the subtraction is exact; the f16 rounding keeps 11
+// of at most 16 bits: 2^-12 relative, an eighth of a bf16 output's own half step.
+__device__ __forceinline__ unsigned q16_to_f16(unsigned w) {
+    w ^= 0x00800080u;
+    const float bias = 8388608.0f + 32768.0f;
+    const float lo = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7601)) - bias;
+    const float hi = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7623)) - bias;
+    return pack_f16(lo, hi);
+}
+// Bytes (already xor 0x80) 0,1 / 2,3 of x as f16 levels: 1024 + u in the
+// mantissa, minus 1152; exact.
+__device__ __forceinline__ unsigned q8_pair(unsigned x, bool high) {
+    const unsigned m = __byte_perm(x, 0x64646464u, high ? 0x4342 : 0x4140);
+    unsigned r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0x64806480u));
+    return r;
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    if (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 16 bytes global -> shared, or 16 zero bytes (src is not read then).
+__device__ __forceinline__ void cp_async16_or_zero(unsigned dst, const void* src, bool live) {
+    const int n = live ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Stores 2 or 1 consecutive floats as `type` at element index i of a row.
+__device__ __forceinline__ void store_as(void* row, int type, long long i, float v) {
+    if (type == VC4_F32) reinterpret_cast<float*>(row)[i] = v;
+    else if (type == VC4_BF16) reinterpret_cast<__nv_bfloat16*>(row)[i] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(row)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ void store4_as(void* row, int type, long long i, float4 v) {
+    if (type == VC4_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(row) + i) = v;
+    else if (type == VC4_BF16)
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(row) + i) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    else
+        *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(row) + i) = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
+}
+
+}  // namespace
+}  // namespace vc4

@@ -190,11 +190,14 @@ int max_input_cols();
 
 // Accessors engine.cu gives the library's other translation units.
 }  // namespace vc4
+struct vc4_gpu;
 struct vc4_model;
 struct vc4_session;
 namespace vc4 {
 int set_error(int code, const char* msg);
 const DModel& model_of(const vc4_model* m);
+int gpu_device(const vc4_gpu* g);
+cudaStream_t gpu_stream(const vc4_gpu* g);
 // What the per-op calls (ops.cu) need of a session.
 struct SessionView {
     State* st;

@@ -19,6 +19,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("VC4B200_LIB") or os.path.join(_HERE, "_lib", "libvc4b200.so")
 
 WQ8, WQ4, WT3 = 0, 1, 2
+DTYPES = {"f32": 0, "bf16": 1, "f16": 2, "q16": 3}          # VC4_F32 .. VC4_Q16I
+PAGE_FORMATS = {"q8": 8, "q16": 16, "bf16": 1, "f16": 2}    # VC4_KV_*
 MATS = {"qkv": 0, "wo": 1, "w1": 2, "w3": 3, "w2": 4, "router": 5, "logits": 6}
 
 
@@ -33,6 +35,16 @@ class ModelInfo(C.Structure):
         "qk_norm", "rope_half", "head_dedup", "wtype")] + [
         ("rope_theta", C.c_float), ("rms_eps", C.c_float),
         ("weight_bytes", C.c_uint64), ("source_size", C.c_uint64), ("source_mtime", C.c_uint64)]
+
+
+class _Pages(C.Structure):
+    _fields_ = [("data", C.c_void_p)] + [(n, C.c_int) for n in (
+        "format", "pages", "page_len", "kv_heads", "head_dim")]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("seqs", "tokens", "max_new", "max_len", "table_stride")] + [
+        (n, C.c_void_p) for n in ("cu", "len", "table", "status")]
 
 
 _lib = None
@@ -92,6 +104,20 @@ _PROTOS = {
     "vc4_logits_from": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "vc4_logits_argmax_from": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int)]),
     "vc4_read_buffer": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "vc4_paged_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_int,
+                                   C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                   C.c_void_p, C.c_int, C.c_longlong, C.c_void_p]),
+    "vc4_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_int,
+                                      C.c_float, C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_size_t,
+                                      C.c_void_p]),
+    "vc4_paged_attention_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_size_t)]),
+    "vc4_verify_draft": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                   C.c_longlong, C.c_void_p, C.c_longlong, C.c_float, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                   C.c_void_p]),
+    "vc4_verify_draft_bytes": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    "vc4_step_draft": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_float, C.c_void_p,
+                                 C.c_float, C.c_void_p, C.POINTER(C.c_int), C.c_void_p]),
     "vc4_counters": (C.c_int, [C.c_void_p, C.POINTER(C.c_longlong), C.POINTER(C.c_longlong)]),
     "vc4_launches_per_step": (C.c_int, [C.c_void_p, C.c_int]),
 }
@@ -149,6 +175,23 @@ class GPU:
     def sync(self):
         _check(lib().vc4_gpu_sync(self._h))
 
+    def verify_bytes(self, seqs: int, rows: int, vocab: int) -> int:
+        """Bytes of verify_draft's work buffer."""
+        n = C.c_size_t()
+        _check(lib().vc4_verify_draft_bytes(seqs, rows, vocab, C.byref(n)))
+        return n.value
+
+    def verify_draft(self, seqs: int, rows: int, vocab: int, cu: int, fed: int, logits: int, logits_type: str,
+                     temperature: float, u: int, u_sample: int, next_tokens: int, accepted: int, prob: int, work: int,
+                     work_bytes: int, probs: int = 0, logits_stride: int = 0, probs_stride: int = 0, status: int = 0,
+                     stream: int = 0):
+        """Which drafted tokens stand and the sampled token behind them
+        (vc4_verify_draft).  Arrays are raw device pointers as ints, 0 where an
+        optional one is absent; logits_type "f32", "bf16", "f16" or "q16"."""
+        _check(lib().vc4_verify_draft(self._h, seqs, rows, vocab, cu, fed, logits, _dtype(logits_type), logits_stride,
+                                      probs, probs_stride, temperature, u, u_sample, next_tokens, accepted, prob,
+                                      status, work, work_bytes, stream))
+
     def close(self):
         if self._h:
             lib().vc4_gpu_destroy(self._h)
@@ -159,6 +202,60 @@ class GPU:
             self.close()
         except Exception:
             pass
+
+
+def _dtype(name: str) -> int:
+    try:
+        return DTYPES[name]
+    except KeyError:
+        raise EngineError("unknown element type %r (one of %s)" % (name, ", ".join(DTYPES))) from None
+
+
+class PagedBatch:
+    """Some new tokens of several sequences over a paged cache
+    (vc4_paged_batch): raw device pointers of int32 arrays as ints, and the
+    bounds that choose the launch."""
+
+    def __init__(self, cu: int, length: int, table: int, seqs: int, tokens: int, max_new: int, max_len: int,
+                 table_stride: int, status: int = 0):
+        self._c = _PagedBatch(seqs, tokens, max_new, max_len, table_stride, cu, length, table, status)
+        self._p = C.addressof(self._c)
+
+
+class PagedKV:
+    """A pool of KV pages the caller owns (vc4_pages): `data` is the raw device
+    pointer of [pages][K, V][kv_heads][page_len][head_dim] values; fmt "q8" and
+    "q16" are the slot cache's codec, "bf16" and "f16" plain floats.  A model with
+    several layers has one pool per layer."""
+
+    def __init__(self, gpu: GPU, data: int, fmt: str, pages: int, page_len: int, kv_heads: int, head_dim: int):
+        if fmt not in PAGE_FORMATS:
+            raise EngineError("unknown page format %r (one of %s)" % (fmt, ", ".join(PAGE_FORMATS)))
+        self.gpu = gpu
+        self._c = _Pages(data, PAGE_FORMATS[fmt], pages, page_len, kv_heads, head_dim)
+        self._p = C.addressof(self._c)
+
+    def append(self, batch: PagedBatch, qkv: int, qkv_type: str, heads: int, q: int, q_type: str, q_norm: int = 0,
+               k_norm: int = 0, eps: float = 1e-6, cos: int = 0, sin: int = 0, rope_len: int = 0,
+               rope_half: bool = True, qkv_stride: int = 0, q_stride: int = 0, stream: int = 0):
+        """Write the new tokens' K and V, normalised and rotated, into their
+        pages and the rotated q rows to `q` (vc4_paged_append)."""
+        _check(lib().vc4_paged_append(self.gpu._h, self._p, batch._p, qkv, _dtype(qkv_type), qkv_stride, heads, q_norm,
+                                      k_norm, eps, cos, sin, rope_len, 1 if rope_half else 0, q, _dtype(q_type),
+                                      q_stride, stream))
+
+    def attend_bytes(self, batch: PagedBatch, heads: int) -> int:
+        """Bytes of attend's work buffer for this batch's bounds."""
+        n = C.c_size_t()
+        _check(lib().vc4_paged_attention_bytes(self.gpu._h, self._p, batch._p, heads, C.byref(n)))
+        return n.value
+
+    def attend(self, batch: PagedBatch, q: int, q_type: str, heads: int, out: int, out_type: str, work: int = 0,
+               work_bytes: int = 0, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, stream: int = 0):
+        """Attention of the new tokens over their sequences' pages
+        (vc4_paged_attention)."""
+        _check(lib().vc4_paged_attention(self.gpu._h, self._p, batch._p, q, _dtype(q_type), q_stride, heads, scale, out,
+                                         _dtype(out_type), out_stride, work, work_bytes, stream))
 
 
 class Model:
@@ -267,6 +364,29 @@ class Session:
         out = np.empty((len(t), self.vocab), np.float32)
         _check(lib().vc4_prefill_logits(self._h, slot, _p(t), len(t), pos0, _p(out)))
         return out
+
+    def step_draft(self, tokens, pos0: int, draft_probs=None, temperature: float = 0.0, u=None, u_sample: float = 0.0,
+                   slot: int = 0):
+        """One speculative step (vc4_step_draft): tokens[0] is the last token,
+        the others its drafts, fed from pos0; draft_probs (drafts x vocab) is
+        what they were sampled from (None: chosen outright), u one random number
+        per draft.  Returns (tokens gained: accepted drafts and the one that
+        follows, their target probabilities)."""
+        t = np.ascontiguousarray(tokens, np.int32)
+        n = len(t)
+        un = np.zeros(max(1, n - 1), np.float32) if u is None else np.ascontiguousarray(u, np.float32)
+        if n > 1 and (un.ndim != 1 or len(un) < n - 1 or (u is None and temperature > 0)):
+            raise EngineError("step_draft: one random number per draft is needed")
+        dp = None
+        if draft_probs is not None:
+            dp = np.ascontiguousarray(draft_probs, np.float32)
+            if dp.shape != (n - 1, self.vocab):
+                raise EngineError("step_draft: draft_probs must be drafts x vocab")
+        nxt, prob, acc = np.empty(max(1, n), np.int32), np.empty(max(1, n), np.float32), C.c_int()
+        _check(lib().vc4_step_draft(self._h, slot, _p(t), n, pos0, _p(dp) if dp is not None and n > 1 else None,
+                                    temperature, _p(un), u_sample, _p(nxt), C.byref(acc), _p(prob)))
+        k = acc.value + 1
+        return [int(v) for v in nxt[:k]], prob[:k].copy()
 
     # -- KV rows and the MMKV1 prefix cache ---------------------------------
     def kv_row_bytes(self) -> int:
