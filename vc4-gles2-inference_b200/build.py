@@ -25,7 +25,7 @@ FLAGS = ["-std=c++17", "-O3", "-lineinfo", "--fmad=false", "-I" + INCLUDE, "-I" 
          "-Xcompiler", "-fPIC,-ffp-contract=off,-fvisibility=hidden", "-diag-suppress", "177"]
 SOURCES = ["kernels.cu", "ops_q8.cu", "ops_q4.cu", "ops_t3.cu", "engine.cu", "noalloc.cu", "ops.cu",
            "paged.cu", "paged_q8.cu", "paged_q16.cu", "paged_bf16.cu", "paged_f16.cu", "verify.cu", "mmcf.cpp"]
-HEADERS = ["vc4b200_internal.h", "kernels.cuh", "batch.cuh", "ops_wt.inc", "paged.cuh", "paged_split.inc"]
+HEADERS = ["vc4b200_internal.h", "kernels.cuh", "batch.cuh", "ops_wt.inc", "paged.cuh", "paged_split.inc", "paged_chunk.inc"]
 
 
 def _newer(target: str, deps: list) -> bool:

@@ -307,22 +307,29 @@ int pfmt(int format) {
 }
 
 struct AttnPlan {
+    bool chunk;           // the many-row kernel
     int wr, row_tiles, splits;
     size_t bytes;
 };
 
-// Rows of a block: the least of 16, 32 and 64 that holds one sequence's rows.
-// Splits: enough blocks for two on each of the GPU's SMs, but at least two tiles
-// of 64 positions each (a split costs a partial result and a second kernel).
-AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms) {
+// Up to 64 rows (new tokens x query heads of a KV head) of a sequence go to the
+// split kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
+// the many-row kernel, 256 a block.  q16 pages with an f16 or float output stay
+// with the split kernel, which holds a level in two operands.
+// Splits: enough blocks for two on each of the GPU's SMs (one of the many-row
+// kernel), but at least two tiles of 64 positions each (eight of 128): a split costs
+// a partial result and a second kernel.
+AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
     const long long rows = (long long)b->max_new * (heads / p->kv_heads);
+    pl.chunk = rows > 64 && !(p->format == VC4_KV_Q16 && out_type != VC4_BF16);
     pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    pl.row_tiles = (int)((rows + 16 * pl.wr - 1) / (16 * pl.wr));
+    const int per = pl.chunk ? 256 : 16 * pl.wr, tile = pl.chunk ? 128 : kPagedTile;
+    pl.row_tiles = (int)((rows + per - 1) / per);
     const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
-    const int tiles = (b->max_len + kPagedTile - 1) / kPagedTile;
-    const long long want = (2 * (long long)sms + units - 1) / units;
-    pl.splits = (int)std::max(1LL, std::min({want, (long long)tiles / 2, (long long)kPagedMaxSplits}));
+    const int tiles = (b->max_len + tile - 1) / tile;
+    const long long want = ((pl.chunk ? 1 : 2) * (long long)sms + units - 1) / units;
+    pl.splits = (int)std::max(1LL, std::min({want, (long long)tiles / (pl.chunk ? 8 : 2), (long long)kPagedMaxSplits}));
     if (pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
     return pl;
 }
@@ -404,7 +411,7 @@ extern "C" int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const v
     if (!g) return refuse("gpu is null");
     int sms = 0;
     if (int e = sms_of(gpu_device(g), &sms)) return e;
-    *bytes = attn_plan(p, b, heads, sms).bytes;
+    *bytes = std::max(attn_plan(p, b, heads, sms, VC4_BF16).bytes, attn_plan(p, b, heads, sms, VC4_F32).bytes);
     return VC4_OK;
 }
 
@@ -430,7 +437,7 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
     if (!g) return refuse("gpu is null");
     int sms = 0;
     if (int e = sms_of(gpu_device(g), &sms)) return e;
-    const AttnPlan pl = attn_plan(p, b, heads, sms);
+    const AttnPlan pl = attn_plan(p, b, heads, sms, out_type);
     if (work_bytes < pl.bytes || (pl.bytes && (!work || !aligned16(work))))
         return refuse("the work buffer needs " + std::to_string(pl.bytes) + " bytes at a multiple of 16");
     if (!b->tokens || !b->max_new) return VC4_OK;
@@ -450,7 +457,16 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
         a.part = (float*)work;
         a.ml = (float2*)((char*)work + (size_t)pl.splits * b->tokens * heads * p->head_dim * 4);
     }
-    switch (pfmt(p->format)) {
+    if (pl.chunk) {
+        bool ok;
+        switch (pfmt(p->format)) {
+            case P_Q8: ok = launch_paged_chunk_q8(a, st); break;
+            case P_Q16: ok = launch_paged_chunk_q16(a, st); break;
+            case P_BF16: ok = launch_paged_chunk_bf16(a, st); break;
+            default: ok = launch_paged_chunk_f16(a, st); break;
+        }
+        if (!ok) return fail(VC4_ECUDA, "paged_attention: no TMA descriptor for this pool");
+    } else switch (pfmt(p->format)) {
         case P_Q8: launch_paged_split_q8(a, pl.wr, st); break;
         case P_Q16: launch_paged_split_q16(a, pl.wr, st); break;
         case P_BF16: launch_paged_split_bf16(a, pl.wr, st); break;

@@ -42,6 +42,11 @@ void launch_paged_split_q8(const PagedAttnArgs& a, int wr, cudaStream_t st);
 void launch_paged_split_q16(const PagedAttnArgs& a, int wr, cudaStream_t st);
 void launch_paged_split_bf16(const PagedAttnArgs& a, int wr, cudaStream_t st);
 void launch_paged_split_f16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+// The many-row kernels; false where no TMA descriptor of the pool can be made.
+bool launch_paged_chunk_q8(const PagedAttnArgs& a, cudaStream_t st);
+bool launch_paged_chunk_q16(const PagedAttnArgs& a, cudaStream_t st);
+bool launch_paged_chunk_bf16(const PagedAttnArgs& a, cudaStream_t st);
+bool launch_paged_chunk_f16(const PagedAttnArgs& a, cudaStream_t st);
 
 namespace {
 
@@ -105,13 +110,23 @@ __device__ __forceinline__ unsigned bf16_to_f16(unsigned w) {
 }
 // Two q16 levels (big-endian int16 in memory) as f16: 2^23 + (level + 2^15)
 // built in the mantissa, so the subtraction is exact; the f16 rounding keeps 11
-// of at most 16 bits: 2^-12 relative, an eighth of a bf16 output's own half step.
-__device__ __forceinline__ unsigned q16_to_f16(unsigned w) {
+// of at most 16 bits (2^-12 relative), and `rest` what it drops, exactly.
+template <bool REST>
+__device__ __forceinline__ unsigned q16_to_f16(unsigned w, unsigned& rest) {
     w ^= 0x00800080u;
     const float bias = 8388608.0f + 32768.0f;
     const float lo = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7601)) - bias;
     const float hi = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7623)) - bias;
-    return pack_f16(lo, hi);
+    const unsigned r = pack_f16(lo, hi);
+    if (REST) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        rest = pack_f16(lo - f.x, hi - f.y);
+    }
+    return r;
+}
+__device__ __forceinline__ unsigned q16_to_f16(unsigned w) {
+    unsigned none;
+    return q16_to_f16<false>(w, none);
 }
 // Bytes (already xor 0x80) 0,1 / 2,3 of x as f16 levels: 1024 + u in the
 // mantissa, minus 1152; exact.
