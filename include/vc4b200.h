@@ -308,7 +308,8 @@ VC4_API int vc4_read_buffer(vc4_session* s, int slot, int buf, int n, float* out
    caller hands out, and the decision on drafted tokens that a verification pass
    of the target model ends with.  All arrays are the caller's device buffers on
    the GPU of `g`.  Nothing is allocated, freed or kept between calls: the work is
-   queued on `stream` (NULL: the stream of `g`) and the call returns without
+   queued on `stream` (NULL: the stream of `g`; CUDA's default stream is
+   cudaStreamLegacy) and the call returns without
    waiting, so it may be captured into a CUDA graph (make one call of the same
    shape before the capture, as with every kernel of this library).  Calls on
    different streams may overlap when their outputs and work buffers are

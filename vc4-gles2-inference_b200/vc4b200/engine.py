@@ -184,13 +184,13 @@ class GPU:
     def verify_draft(self, seqs: int, rows: int, vocab: int, cu: int, fed: int, logits: int, logits_type: str,
                      temperature: float, u: int, u_sample: int, next_tokens: int, accepted: int, prob: int, work: int,
                      work_bytes: int, probs: int = 0, logits_stride: int = 0, probs_stride: int = 0, status: int = 0,
-                     stream: int = 0):
+                     stream: int = None):
         """Which drafted tokens stand and the sampled token behind them
         (vc4_verify_draft).  Arrays are raw device pointers as ints, 0 where an
         optional one is absent; logits_type "f32", "bf16", "f16" or "q16"."""
         _check(lib().vc4_verify_draft(self._h, seqs, rows, vocab, cu, fed, logits, _dtype(logits_type), logits_stride,
                                       probs, probs_stride, temperature, u, u_sample, next_tokens, accepted, prob,
-                                      status, work, work_bytes, stream))
+                                      status, work, work_bytes, _stream(stream)))
 
     def close(self):
         if self._h:
@@ -209,6 +209,12 @@ def _dtype(name: str) -> int:
         return DTYPES[name]
     except KeyError:
         raise EngineError("unknown element type %r (one of %s)" % (name, ", ".join(DTYPES))) from None
+
+
+def _stream(stream):
+    """A CUDA stream handle for the C ABI: None is the GPU handle's own stream
+    (NULL there), 0 CUDA's default stream (cudaStreamLegacy), as in torch."""
+    return None if stream is None else stream or 1
 
 
 class PagedBatch:
@@ -237,12 +243,12 @@ class PagedKV:
 
     def append(self, batch: PagedBatch, qkv: int, qkv_type: str, heads: int, q: int, q_type: str, q_norm: int = 0,
                k_norm: int = 0, eps: float = 1e-6, cos: int = 0, sin: int = 0, rope_len: int = 0,
-               rope_half: bool = True, qkv_stride: int = 0, q_stride: int = 0, stream: int = 0):
+               rope_half: bool = True, qkv_stride: int = 0, q_stride: int = 0, stream: int = None):
         """Write the new tokens' K and V, normalised and rotated, into their
         pages and the rotated q rows to `q` (vc4_paged_append)."""
         _check(lib().vc4_paged_append(self.gpu._h, self._p, batch._p, qkv, _dtype(qkv_type), qkv_stride, heads, q_norm,
                                       k_norm, eps, cos, sin, rope_len, 1 if rope_half else 0, q, _dtype(q_type),
-                                      q_stride, stream))
+                                      q_stride, _stream(stream)))
 
     def attend_bytes(self, batch: PagedBatch, heads: int) -> int:
         """Bytes of attend's work buffer for this batch's bounds."""
@@ -251,11 +257,11 @@ class PagedKV:
         return n.value
 
     def attend(self, batch: PagedBatch, q: int, q_type: str, heads: int, out: int, out_type: str, work: int = 0,
-               work_bytes: int = 0, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, stream: int = 0):
+               work_bytes: int = 0, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, stream: int = None):
         """Attention of the new tokens over their sequences' pages
         (vc4_paged_attention)."""
         _check(lib().vc4_paged_attention(self.gpu._h, self._p, batch._p, q, _dtype(q_type), q_stride, heads, scale, out,
-                                         _dtype(out_type), out_stride, work, work_bytes, stream))
+                                         _dtype(out_type), out_stride, work, work_bytes, _stream(stream)))
 
 
 class Model:
