@@ -425,12 +425,12 @@ def test_captured_step_follows_its_arrays(new):
 @pytest.mark.gpu
 def test_no_tokens_and_work_buffer():
     gpu = vc4b200.GPU(0)
-    cache = Cache([5000], [1], "q8", 16, 2, 64)
+    cache = Cache([5000], [100], "q8", 16, 2, 64)
     handle, batch = cache.handles(vc4b200, gpu)
     need = handle.attend_bytes(batch, 4)
     assert need > 0
-    q = torch.randn(1, 256, device="cuda").to(torch.bfloat16)
-    out = torch.zeros(1, 256, device="cuda")
+    q = torch.randn(100, 256, device="cuda").to(torch.bfloat16)
+    out = torch.zeros(100, 256, device="cuda")
     _refused(lambda: handle.attend(batch, q.data_ptr(), "bf16", 4, out.data_ptr(), "f32", out.data_ptr(), need - 1), "work buffer")
     _refused(lambda: handle.attend(batch, q.data_ptr(), "bf16", 4, out.data_ptr(), "f32", 0, need), "work buffer")
     empty = vc4b200.PagedBatch(cache.cu.data_ptr(), cache.len.data_ptr(), cache.table.data_ptr(), 1, 0, 0, 0, cache.width)

@@ -313,24 +313,26 @@ struct AttnPlan {
 };
 
 // Up to 64 rows (new tokens x query heads of a KV head) of a sequence go to the
-// split kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
+// few-row kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
 // the many-row kernel, 256 a block.  q16 pages with an f16 or float output stay
-// with the split kernel, which holds a level in two operands.
-// Splits: enough blocks for two on each of the GPU's SMs (one of the many-row
-// kernel), but at least two tiles of 64 positions each (eight of 128): a split costs
-// a partial result and a second kernel.
+// with the few-row kernel, which holds a level in two operands.
+// Splits: enough blocks for three on each of the GPU's SMs (one of the many-row
+// kernel), but at least two tiles of 64 positions each (eight of 128).  The few-row
+// kernel's are a cluster; the many-row kernel's leave partial results in the work
+// buffer, for a second kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
     const long long rows = (long long)b->max_new * (heads / p->kv_heads);
     pl.chunk = rows > 64 && !(p->format == VC4_KV_Q16 && out_type != VC4_BF16);
     pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const int per = pl.chunk ? 256 : 16 * pl.wr, tile = pl.chunk ? 128 : kPagedTile;
+    const int per = pl.chunk ? 256 : 16 * pl.wr, tile = pl.chunk ? 128 : 64;
     pl.row_tiles = (int)((rows + per - 1) / per);
     const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
     const int tiles = (b->max_len + tile - 1) / tile;
-    const long long want = ((pl.chunk ? 1 : 2) * (long long)sms + units - 1) / units;
-    pl.splits = (int)std::max(1LL, std::min({want, (long long)tiles / (pl.chunk ? 8 : 2), (long long)kPagedMaxSplits}));
-    if (pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
+    const long long want = ((pl.chunk ? 1 : 3) * (long long)sms + (pl.chunk ? units - 1 : 0)) / units;
+    pl.splits = (int)std::max(1LL, std::min({want, (long long)tiles / (pl.chunk ? 8 : 2),
+                                             (long long)(pl.chunk ? kPagedMaxSplits : kPagedMaxCluster)}));
+    if (pl.chunk && pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
     return pl;
 }
 
@@ -453,26 +455,19 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
     const double sc = scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)p->head_dim);
     a.scale2 = (float)(sc * 1.4426950408889634 * grid);
     a.vscale = (float)grid;
-    if (pl.splits > 1) {
+    if (pl.bytes) {
         a.part = (float*)work;
         a.ml = (float2*)((char*)work + (size_t)pl.splits * b->tokens * heads * p->head_dim * 4);
     }
-    if (pl.chunk) {
-        bool ok;
-        switch (pfmt(p->format)) {
-            case P_Q8: ok = launch_paged_chunk_q8(a, st); break;
-            case P_Q16: ok = launch_paged_chunk_q16(a, st); break;
-            case P_BF16: ok = launch_paged_chunk_bf16(a, st); break;
-            default: ok = launch_paged_chunk_f16(a, st); break;
-        }
-        if (!ok) return fail(VC4_ECUDA, "paged_attention: no TMA descriptor for this pool");
-    } else switch (pfmt(p->format)) {
-        case P_Q8: launch_paged_split_q8(a, pl.wr, st); break;
-        case P_Q16: launch_paged_split_q16(a, pl.wr, st); break;
-        case P_BF16: launch_paged_split_bf16(a, pl.wr, st); break;
-        default: launch_paged_split_f16(a, pl.wr, st); break;
+    bool ok;
+    switch (pfmt(p->format)) {
+        case P_Q8: ok = pl.chunk ? launch_paged_chunk_q8(a, st) : launch_paged_split_q8(a, pl.wr, st); break;
+        case P_Q16: ok = pl.chunk ? launch_paged_chunk_q16(a, st) : launch_paged_split_q16(a, pl.wr, st); break;
+        case P_BF16: ok = pl.chunk ? launch_paged_chunk_bf16(a, st) : launch_paged_split_bf16(a, pl.wr, st); break;
+        default: ok = pl.chunk ? launch_paged_chunk_f16(a, st) : launch_paged_split_f16(a, pl.wr, st); break;
     }
-    if (pl.splits > 1) launch_pdl_block(k_paged_join, dim3((unsigned)b->tokens), 128, 0, st, a);
+    if (!ok) return fail(VC4_ECUDA, "paged_attention: no TMA descriptor for this pool");
+    if (pl.bytes) launch_pdl_block(k_paged_join, dim3((unsigned)b->tokens), 128, 0, st, a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return fail(VC4_ECUDA, std::string("paged_attention: ") + cudaGetErrorString(e));
     return VC4_OK;

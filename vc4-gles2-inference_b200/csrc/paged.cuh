@@ -33,15 +33,15 @@ struct PagedAttnArgs {
     int row_tiles, splits;   // grid: ((sequence * kv_heads + head) * row_tiles + tile) * splits + split
     float scale2;            // score scale x log2 e x the K grid
     float vscale;            // the V grid
-    float* part;             // [splits][tokens*heads][head_dim] unnormalised sums
+    float* part;             // many-row kernel: [splits][tokens*heads][head_dim] unnormalised sums
     float2* ml;              // [splits][tokens*heads] running maximum (of the unscaled score) and sum
 };
 
 // The split kernels of one format (paged_*.cu); wr: 16-row tiles per block (1, 2 or 4).
-void launch_paged_split_q8(const PagedAttnArgs& a, int wr, cudaStream_t st);
-void launch_paged_split_q16(const PagedAttnArgs& a, int wr, cudaStream_t st);
-void launch_paged_split_bf16(const PagedAttnArgs& a, int wr, cudaStream_t st);
-void launch_paged_split_f16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+bool launch_paged_split_q8(const PagedAttnArgs& a, int wr, cudaStream_t st);
+bool launch_paged_split_q16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+bool launch_paged_split_bf16(const PagedAttnArgs& a, int wr, cudaStream_t st);
+bool launch_paged_split_f16(const PagedAttnArgs& a, int wr, cudaStream_t st);
 // The many-row kernels; false where no TMA descriptor of the pool can be made.
 bool launch_paged_chunk_q8(const PagedAttnArgs& a, cudaStream_t st);
 bool launch_paged_chunk_q16(const PagedAttnArgs& a, cudaStream_t st);
@@ -50,9 +50,8 @@ bool launch_paged_chunk_f16(const PagedAttnArgs& a, cudaStream_t st);
 
 namespace {
 
-constexpr int kPagedSplitThreads = 128;
-constexpr int kPagedTile = 64;      // positions per K/V tile of the split kernels
-constexpr int kPagedMaxSplits = 64;
+constexpr int kPagedMaxSplits = 64;    // of the many-row kernel
+constexpr int kPagedMaxCluster = 8;    // splits of the few-row kernel: blocks of a cluster
 
 __device__ __forceinline__ void paged_flag(int* status, int code) {
     if (status) atomicMax(status, code);
@@ -149,14 +148,18 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const unsigned (&a)[4],
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16 bytes global -> shared, or 16 zero bytes (src is not read then).
-__device__ __forceinline__ void cp_async16_or_zero(unsigned dst, const void* src, bool live) {
-    const int n = live ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// The pool as rows of `row_bytes`; a box is `width` bytes of as many rows as a page has
+// in a tile.  False where no descriptor can be made.
+inline bool paged_map(CUtensorMap* map, const PagedArgs& p, int row_bytes, int width, int tile, CUtensorMapSwizzle swizzle) {
+    const auto enc = tmap_encode_fn();
+    const int page_len = 1 << p.page_shift, span = page_len < tile ? page_len : tile;
+    const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, ((cuuint64_t)p.pages * 2 * p.kv_heads) << p.page_shift};
+    const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)span}, es[2] = {1, 1};
+    return enc && dims[1] <= 0x7fffffffull &&
+           enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.data, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Stores 2 or 1 consecutive floats as `type` at element index i of a row.
 __device__ __forceinline__ void store_as(void* row, int type, long long i, float v) {
