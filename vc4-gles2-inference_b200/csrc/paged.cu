@@ -316,10 +316,12 @@ struct AttnPlan {
 // few-row kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
 // the many-row kernel, 256 a block.  q16 pages with an f16 or float output stay
 // with the few-row kernel, which holds a level in two operands.
-// Splits: enough blocks for three on each of the GPU's SMs (one of the many-row
-// kernel), but at least two tiles of 64 positions each (eight of 128).  The few-row
-// kernel's are a cluster; the many-row kernel's leave partial results in the work
-// buffer, for a second kernel.
+// Splits of the few-row kernel (a power of two: a cluster's blocks lie in one GPC): as
+// many as the GPU holds at once, of two tiles of 64 positions or more; twice that or
+// more of long sequences, whose ragged lengths then even out (12 x 40k positions: 1, 2, 4,
+// 8 splits 457, 274, 278, 244 us).  Of the many-row kernel: a block on every SM, of
+// eight tiles of 128 or more; they leave partial results in the work buffer, for a second
+// kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
     const long long rows = (long long)b->max_new * (heads / p->kv_heads);
@@ -329,9 +331,15 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
     pl.row_tiles = (int)((rows + per - 1) / per);
     const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
     const int tiles = (b->max_len + tile - 1) / tile;
-    const long long want = ((pl.chunk ? 1 : 3) * (long long)sms + (pl.chunk ? units - 1 : 0)) / units;
-    pl.splits = (int)std::max(1LL, std::min({want, (long long)tiles / (pl.chunk ? 8 : 2),
-                                             (long long)(pl.chunk ? kPagedMaxSplits : kPagedMaxCluster)}));
+    if (pl.chunk) {
+        pl.splits = (int)std::max(1LL, std::min({(sms + units - 1) / units, (long long)tiles / 8, (long long)kPagedMaxSplits}));
+    } else {
+        const int es = p->format == VC4_KV_Q8 ? 1 : 2;
+        const long long fit = (long long)sms * split_blocks(es, p->head_dim, pl.wr);
+        pl.splits = 1;
+        while (pl.splits < kPagedMaxCluster && 2 * pl.splits * units <= fit && tiles >= 4 * pl.splits) pl.splits *= 2;
+        while (pl.splits < kPagedMaxCluster && pl.splits * units * 2 > fit && units < fit && tiles >= 128 * pl.splits) pl.splits *= 2;
+    }
     if (pl.chunk && pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
     return pl;
 }

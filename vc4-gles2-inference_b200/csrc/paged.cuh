@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 namespace vc4 {
 
 // Formats as template arguments.
@@ -146,6 +148,36 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const unsigned (&a)[4],
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---- the few-row kernel's tiles (es: bytes of a cached value) ----
+
+// How a tile lies in shared memory.  Rows of 128 bytes (f16, bf16 from head size 64 in
+// panels of 64 values; q8 of 128) are in the 128-byte swizzle and rows of 64 (q8) in the
+// 64-byte one, so that the lanes' fragment loads spread over the banks; the others are
+// packed.
+__host__ __device__ constexpr int split_mode(int es, int hd) {   // 0 packed, 1 128-byte, 2 64-byte swizzle
+    return es == 2 ? (hd >= 64 ? 1 : 0) : hd == 128 ? 1 : hd == 64 ? 2 : 0;
+}
+__host__ __device__ constexpr int split_panels(int es, int hd) { return es == 2 && hd > 64 ? 2 : 1; }
+__host__ __device__ constexpr int split_pitch(int es, int hd) { return split_mode(es, hd) == 1 ? 128 : hd * es; }
+// positions per tile: 128 for short rows of the 16-row kernel (a tile's softmax and
+// barriers cost the same for 16 and 32 positions of a warp)
+__host__ __device__ constexpr int split_tile(int es, int hd, int wr) { return wr == 1 && hd * es <= 128 ? 128 : 64; }
+__host__ __device__ constexpr int split_half(int es, int hd, int wr) { return split_tile(es, hd, wr) * split_pitch(es, hd) * split_panels(es, hd); }
+__host__ __device__ constexpr int split_stages(int es, int hd, int wr) {   // about 75 KB: three blocks on an SM
+    const int s = (75 * 1024) / (2 * split_half(es, hd, wr));
+    return s < 3 ? 3 : s > 6 ? 6 : s;
+}
+__host__ __device__ constexpr size_t split_smem(int es, int hd, int wr) {
+    const size_t ring = (size_t)2 * split_half(es, hd, wr) * split_stages(es, hd, wr), join = 4 * 16 * (size_t)(hd + 4) * 4 + 4 * 16 * 8;
+    return 1023 + (ring > join ? ring : join);      // 1023: the ring starts on a swizzle atom
+}
+
+// Blocks of the kernel an SM holds: by its launch bounds and by shared memory.
+__host__ __device__ constexpr int split_bound(int es, int hd, int wr) { return hd * wr <= 64 ? 4 : wr == 4 && hd >= 96 ? 2 : 3; }
+inline int split_blocks(int es, int hd, int wr) {
+    return std::max(1, std::min(split_bound(es, hd, wr), (int)(228 * 1024 / (split_smem(es, hd, wr) + 1024))));
 }
 
 // The pool as rows of `row_bytes`; a box is `width` bytes of as many rows as a page has
