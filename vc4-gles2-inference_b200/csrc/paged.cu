@@ -41,18 +41,36 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 8;    // most tokens of a block (one warp looks one up)
+constexpr int kAppendVecs = 4;      // head vectors a group of lanes holds at once
 
-// Four consecutive values of a row as floats.
+// Four consecutive values of a row, as they lie there and as two float pairs.
+template <int TIN> struct Raw4 { uint2 w; };
+template <> struct Raw4<VC4_F32> { uint4 w; };
 template <int TIN>
-__device__ __forceinline__ float4 load4(const void* row, long long i) {
-    if (TIN == VC4_F32) return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + i);
-    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(row) + i);
-    if (TIN == VC4_BF16)
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
-                           __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    return make_float4(a.x, a.y, b.x, b.y);
+__device__ __forceinline__ void load4(const void* row, long long i, Raw4<TIN>& v) {
+    if constexpr (TIN == VC4_F32) v.w = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(row) + i));
+    else v.w = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(row) + i));
+}
+template <int TIN>
+__device__ __forceinline__ void pairs4(const Raw4<TIN>& r, unsigned long long (&v)[2]) {
+    if constexpr (TIN == VC4_F32) {
+        v[0] = pack2(__uint_as_float(r.w.x), __uint_as_float(r.w.y));
+        v[1] = pack2(__uint_as_float(r.w.z), __uint_as_float(r.w.w));
+    } else if constexpr (TIN == VC4_BF16) {
+        v[0] = pack2(__uint_as_float(r.w.x << 16), __uint_as_float(r.w.x & 0xFFFF0000u));
+        v[1] = pack2(__uint_as_float(r.w.y << 16), __uint_as_float(r.w.y & 0xFFFF0000u));
+    } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.w.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&r.w.y));
+        v[0] = pack2(a.x, a.y);
+        v[1] = pack2(b.x, b.y);
+    }
+}
+__device__ __forceinline__ float4 as_float4(const unsigned long long (&v)[2]) {
+    float4 f;
+    unpack2(v[0], f.x, f.y);
+    unpack2(v[1], f.z, f.w);
+    return f;
 }
 
 // Four consecutive values of a cached row, in the pages' format.
@@ -71,36 +89,47 @@ __device__ __forceinline__ void store_cache4(uint8_t* row, int i, float4 v) {
     }
 }
 
-// One group of LPV lanes per head vector (hd/8 of them at work): a lane holds
-// eight values as four rotation pairs, so norm, rotation and encoding stay in
-// its registers and every load and store is 4 to 16 bytes wide.  Bound by bytes
-// for many tokens, by the chain offsets -> length -> page id for a few; the first
-// vector's loads are issued before that chain.  The float operations are the slot
-// cache's (k_attn): squares summed in double, 1/sqrt(ss/hd + eps), w*(r*x), the
-// rotation's products and sums rounded one by one, the codec's floor(x*grid + 1/2).
-template <int TIN, int FMT>
+// A group of LPV lanes takes four head vectors of a token at once; a lane holds eight
+// values of each as four rotation pairs, so norm, rotation and encoding stay in its
+// registers and every load and store is 4 to 16 bytes wide.  Bound by bytes for many
+// tokens, by the chain offsets -> length -> page id for a few; the first vectors' loads
+// are issued before that chain.  With one vector at a time the square root, the two
+// divisions and the sums' shuffles, the same for every lane, took as long as the bytes
+// (16384 tokens of 32 + 16 heads of 128 in bf16: 120 us against 78): four
+// vectors' sums are halved across the lanes (10 shuffles for 32), so each lane ends with
+// one vector's and takes its root.
+// The float operations are the slot cache's (k_attn): squares summed in double,
+// 1/sqrt(ss/hd + eps), w*(r*x), the rotation's products and sums rounded one by one, the
+// codec's floor(x*grid + 1/2).  Packed products and sums round like single ones.
+template <int TIN, int FMT, int LPV>
 __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
+    constexpr int N = kAppendVecs, NG = 32 / LPV;   // groups of a warp
     const PagedArgs& p = a.p;
-    const int hd = p.head_dim, half = hd / 2, nvec = a.heads + 2 * p.kv_heads;
+    const int hd = p.head_dim, half = hd / 2, nvec = a.heads + 2 * p.kv_heads, turned = a.heads + p.kv_heads;
     __shared__ int s_pos[kAppendTokens];             // the position, -1: nothing to do
     __shared__ long long s_row[kAppendTokens];       // row index of (page, K, head 0, offset)
-    const int lpv = hd > 64 ? 16 : hd > 32 ? 8 : hd > 16 ? 4 : 2;
     const int tok0 = blockIdx.x * a.per_block, ntok = min(a.per_block, p.tokens - tok0);
-    const int sub = threadIdx.x % lpv, grp = threadIdx.x / lpv, ngrp = kAppendThreads / lpv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPV;
     const bool live = sub * 8 < hd;
     const int i0 = a.half ? 4 * sub : 8 * sub, i1 = a.half ? half + 4 * sub : 8 * sub + 4;
-    const int total = ntok * nvec;
-    auto fetch = [&](int it, float4& x0, float4& x1) {
-        if (it < total && live) {
-            const long long base = (long long)(tok0 + it / nvec) * a.qkv_stride + (long long)(it % nvec) * hd;
-            x0 = load4<TIN>(a.qkv, base + i0);
-            x1 = load4<TIN>(a.qkv, base + i1);
-        }
+    // pieces of four vectors of a token; a warp takes NG of them at a time, in order
+    const int pieces = (nvec + N - 1) / N, total = ntok * pieces, step = kAppendThreads / 32 * NG;
+    Raw4<TIN> raw[N][2];
+    auto fetch = [&](int at) {
+        const int t = at / pieces, vec0 = at % pieces * N;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (at < total && live && vec0 + k < nvec) {
+                const long long base = (long long)(tok0 + t) * a.qkv_stride + (long long)(vec0 + k) * hd;
+                load4<TIN>(a.qkv, base + i0, raw[k][0]);
+                load4<TIN>(a.qkv, base + i1, raw[k][1]);
+            } else {
+                raw[k][0] = raw[k][1] = Raw4<TIN>{};
+            }
     };
-    float4 x0 = make_float4(0, 0, 0, 0), x1 = x0;
-    fetch(grp, x0, x1);
+    const int first = warp * NG + lane / LPV;
+    fetch(first);
 
-    const int warp = threadIdx.x >> 5;
     if (warp < ntok) {
         const int tok = tok0 + warp, s = paged_find(p.cu, p.seqs, tok);
         const int c0 = p.cu[s], c1 = p.cu[s + 1];
@@ -117,11 +146,11 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
                 row = (((long long)page * 2 * p.kv_heads) << p.page_shift) + (pos & (page_len - 1));
             }
             if (bad) {
-                if ((threadIdx.x & 31) == 0) paged_flag(p.status, VC4_EINVAL);
+                if (lane == 0) paged_flag(p.status, VC4_EINVAL);
                 pos = -1;
             }
         }
-        if ((threadIdx.x & 31) == 0) {
+        if (lane == 0) {
             s_pos[warp] = pos;
             s_row[warp] = row;
         }
@@ -129,77 +158,129 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
     __syncthreads();
 
     const int es = FMT == P_Q8 ? 1 : 2;
-    // every lane of a warp runs the same number of rounds (the sums shuffle)
-    for (int it0 = 0; it0 < total; it0 += ngrp) {
-        const int it = it0 + grp;
-        float4 n0 = make_float4(0, 0, 0, 0), n1 = n0;
-        fetch(it + ngrp, n0, n1);
-        const int t = min(it, total - 1) / nvec, vec = min(it, total - 1) % nvec;
-        const int pos = it < total ? s_pos[t] : -1;
+    for (int w = warp * NG; w < total; w += step) {          // (the groups of a warp stay together: the sums shuffle)
+        const int at = w + lane / LPV, t = min(at, total - 1) / pieces, vec0 = min(at, total - 1) % pieces * N;
+        const int pos = at < total ? s_pos[t] : -1;
+        unsigned long long x[N][2][2];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            pairs4<TIN>(raw[k][0], x[k][0]);
+            pairs4<TIN>(raw[k][1], x[k][1]);
+        }
+        fetch(at + step);                                    // on its way during this round
         if (a.q_norm) {
-            double acc = 0.0;
-            acc = fma((double)x0.x, (double)x0.x, acc);   // a product of two floats is exact in double
-            acc = fma((double)x0.y, (double)x0.y, acc);
-            acc = fma((double)x0.z, (double)x0.z, acc);
-            acc = fma((double)x0.w, (double)x0.w, acc);
-            acc = fma((double)x1.x, (double)x1.x, acc);
-            acc = fma((double)x1.y, (double)x1.y, acc);
-            acc = fma((double)x1.z, (double)x1.z, acc);
-            acc = fma((double)x1.w, (double)x1.w, acc);
-            if (!live) acc = 0.0;
-            for (int o = lpv / 2; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-            if (vec < a.heads + p.kv_heads && live) {
-                const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(__double2float_rn(acc), (float)hd), a.eps)));
+            double ss[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                ss[k] = 0.0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 f = as_float4(x[k][h]);     // a product of two floats is exact in double
+                    ss[k] = fma((double)f.x, (double)f.x, ss[k]);
+                    ss[k] = fma((double)f.y, (double)f.y, ss[k]);
+                    ss[k] = fma((double)f.z, (double)f.z, ss[k]);
+                    ss[k] = fma((double)f.w, (double)f.w, ss[k]);
+                }
+            }
+            float r[N];
+            auto root = [&](double sum) {
+                return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(__double2float_rn(sum), (float)hd), a.eps)));
+            };
+            if (LPV >= 4) {      // two vectors' halves change places, then one's; then one is summed
+                const bool up = lane & (LPV / 2), right = lane & (LPV / 4);
+                double keep[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    keep[k] = (up ? ss[2 + k] : ss[k]) + __shfl_xor_sync(0xffffffffu, up ? ss[k] : ss[2 + k], LPV / 2);
+                double one = (right ? keep[1] : keep[0]) + __shfl_xor_sync(0xffffffffu, right ? keep[0] : keep[1], LPV / 4);
+#pragma unroll
+                for (int o = LPV / 8; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+                const float mine = root(one);
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    r[k] = __shfl_sync(0xffffffffu, mine, (lane & ~(LPV - 1)) + (k >> 1) * (LPV / 2) + (k & 1) * (LPV / 4));
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) r[k] = root(ss[k] + __shfl_xor_sync(0xffffffffu, ss[k], 1));
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int vec = vec0 + k;
+                if (vec >= turned || !live) continue;
                 const float* w = vec < a.heads ? a.q_norm : a.k_norm;
                 const float4 w0 = *reinterpret_cast<const float4*>(w + i0), w1 = *reinterpret_cast<const float4*>(w + i1);
-                x0 = make_float4(__fmul_rn(w0.x, __fmul_rn(r, x0.x)), __fmul_rn(w0.y, __fmul_rn(r, x0.y)),
-                                 __fmul_rn(w0.z, __fmul_rn(r, x0.z)), __fmul_rn(w0.w, __fmul_rn(r, x0.w)));
-                x1 = make_float4(__fmul_rn(w1.x, __fmul_rn(r, x1.x)), __fmul_rn(w1.y, __fmul_rn(r, x1.y)),
-                                 __fmul_rn(w1.z, __fmul_rn(r, x1.z)), __fmul_rn(w1.w, __fmul_rn(r, x1.w)));
+                const unsigned long long rr = pack2(r[k], r[k]);
+                x[k][0][0] = mul2(pack2(w0.x, w0.y), mul2(rr, x[k][0][0]));
+                x[k][0][1] = mul2(pack2(w0.z, w0.w), mul2(rr, x[k][0][1]));
+                x[k][1][0] = mul2(pack2(w1.x, w1.y), mul2(rr, x[k][1][0]));
+                x[k][1][1] = mul2(pack2(w1.z, w1.w), mul2(rr, x[k][1][1]));
             }
         }
         if (pos >= 0 && live) {
-            if (a.cos && vec < a.heads + p.kv_heads) {
+            if (a.cos) {
                 const float4 c = *reinterpret_cast<const float4*>(a.cos + (size_t)pos * half + 4 * sub);
                 const float4 s = *reinterpret_cast<const float4*>(a.sin + (size_t)pos * half + 4 * sub);
-                auto turn = [](float& u, float& v, float cc, float ss) {
-                    const float y = __fsub_rn(__fmul_rn(u, cc), __fmul_rn(v, ss));
-                    v = __fadd_rn(__fmul_rn(u, ss), __fmul_rn(v, cc));
+                const unsigned long long c0 = pack2(c.x, c.y), c1 = pack2(c.z, c.w), s0 = pack2(s.x, s.y), s1 = pack2(s.z, s.w);
+                const unsigned long long m0 = pack2(-s.x, -s.y), m1 = pack2(-s.z, -s.w);
+                auto turn = [](unsigned long long& u, unsigned long long& v, unsigned long long cc, unsigned long long sn,
+                               unsigned long long neg) {
+                    const unsigned long long y = add2(mul2(u, cc), mul2(v, neg));   // a c - b s, rounded as that
+                    v = add2(mul2(u, sn), mul2(v, cc));
                     u = y;
                 };
-                if (a.half) {
-                    turn(x0.x, x1.x, c.x, s.x);
-                    turn(x0.y, x1.y, c.y, s.y);
-                    turn(x0.z, x1.z, c.z, s.z);
-                    turn(x0.w, x1.w, c.w, s.w);
-                } else {
-                    turn(x0.x, x0.y, c.x, s.x);
-                    turn(x0.z, x0.w, c.y, s.y);
-                    turn(x1.x, x1.y, c.z, s.z);
-                    turn(x1.z, x1.w, c.w, s.w);
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    if (vec0 + k >= turned) continue;
+                    if (a.half) {
+                        turn(x[k][0][0], x[k][1][0], c0, s0, m0);
+                        turn(x[k][0][1], x[k][1][1], c1, s1, m1);
+                    } else {                                  // neighbours: apart, turned, together again
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float4 f = as_float4(x[k][h]);
+                            unsigned long long u = pack2(f.x, f.z), v = pack2(f.y, f.w);
+                            turn(u, v, h ? c1 : c0, h ? s1 : s0, h ? m1 : m0);
+                            float u0, u1, v0, v1;
+                            unpack2(u, u0, u1);
+                            unpack2(v, v0, v1);
+                            x[k][h][0] = pack2(u0, v0);
+                            x[k][h][1] = pack2(u1, v1);
+                        }
+                    }
                 }
             }
-            if (vec < a.heads) {
-                const long long at = (long long)(tok0 + t) * a.q_stride + (long long)vec * hd;
-                store4_as(a.q, a.q_type, at + i0, x0);
-                store4_as(a.q, a.q_type, at + i1, x1);
-            } else {
-                // heads of K, then of V, lie page_len rows apart
-                uint8_t* row = p.data + (s_row[t] + ((long long)(vec - a.heads) << p.page_shift)) * (hd * es);
-                store_cache4<FMT>(row, i0, x0);
-                store_cache4<FMT>(row, i1, x1);
+            const long long qrow = (long long)(tok0 + t) * a.q_stride;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int vec = vec0 + k;
+                if (vec >= nvec) continue;
+                if (vec < a.heads) {
+                    store4_as(a.q, a.q_type, qrow + (long long)vec * hd + i0, as_float4(x[k][0]));
+                    store4_as(a.q, a.q_type, qrow + (long long)vec * hd + i1, as_float4(x[k][1]));
+                } else {
+                    // heads of K, then of V, lie page_len rows apart
+                    uint8_t* row = p.data + (s_row[t] + ((long long)(vec - a.heads) << p.page_shift)) * (hd * es);
+                    store_cache4<FMT>(row, i0, as_float4(x[k][0]));
+                    store_cache4<FMT>(row, i1, as_float4(x[k][1]));
+                }
             }
         }
-        x0 = n0;
-        x1 = n1;
     }
 }
 
+template <int FMT, int LPV>
+void launch_append_lanes(const AppendArgs& a, int type, unsigned blocks, cudaStream_t st) {
+    if (type == VC4_F32) k_paged_append<VC4_F32, FMT, LPV><<<blocks, kAppendThreads, 0, st>>>(a);
+    else if (type == VC4_BF16) k_paged_append<VC4_BF16, FMT, LPV><<<blocks, kAppendThreads, 0, st>>>(a);
+    else k_paged_append<VC4_F16, FMT, LPV><<<blocks, kAppendThreads, 0, st>>>(a);
+}
 template <int FMT>
 void launch_append(const AppendArgs& a, int type, unsigned blocks, cudaStream_t st) {
-    if (type == VC4_F32) k_paged_append<VC4_F32, FMT><<<blocks, kAppendThreads, 0, st>>>(a);
-    else if (type == VC4_BF16) k_paged_append<VC4_BF16, FMT><<<blocks, kAppendThreads, 0, st>>>(a);
-    else k_paged_append<VC4_F16, FMT><<<blocks, kAppendThreads, 0, st>>>(a);
+    const int hd = a.p.head_dim;
+    if (hd > 64) launch_append_lanes<FMT, 16>(a, type, blocks, st);
+    else if (hd > 32) launch_append_lanes<FMT, 8>(a, type, blocks, st);
+    else if (hd > 16) launch_append_lanes<FMT, 4>(a, type, blocks, st);
+    else launch_append_lanes<FMT, 2>(a, type, blocks, st);
 }
 
 // ---------------------------------------------------------------------------
