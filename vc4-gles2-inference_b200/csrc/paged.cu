@@ -287,56 +287,61 @@ void launch_append(const AppendArgs& a, int type, unsigned blocks, cudaStream_t 
 // join of split attention: o = sum_i 2^(c(m_i - m)) O_i / sum_i 2^(c(m_i - m)) l_i
 // ---------------------------------------------------------------------------
 
-// One warp per (token, head); lane i holds the weights of splits i and i + 32.
-__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a) {
+// One warp per (token, head); lane i holds the weights of splits i and i + 32, then four
+// values of the row.
+__global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
     pdl_wait();
-    const int tok = blockIdx.x, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
+    const long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const PagedArgs& p = a.p;
-    const int last = min(p.cu[p.seqs], p.tokens);
-    if (tok >= last) return;
-    // rows of a sequence beyond max_new were not computed: leave them
+    const int tok = (int)(task / a.heads), head = (int)(task % a.heads);
+    if (tok >= p.tokens) return;
+    const size_t at = (size_t)task, step = (size_t)p.tokens * a.heads;
+    float2 e[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        e[k] = lane + 32 * k < a.splits ? a.ml[at + (lane + 32 * k) * step] : make_float2(-INFINITY, 0.0f);
+    // rows behind the last sequence, and those beyond max_new, were not computed: leave them
     const int s = paged_find(p.cu, p.seqs, tok);
     if (tok < p.cu[s] || tok >= p.cu[s + 1] || tok - p.cu[s] >= p.max_new) return;
-    const int hd = p.head_dim;
-    for (int head = threadIdx.x >> 5; head < a.heads; head += blockDim.x >> 5) {
-        const size_t at = (size_t)tok * a.heads + head, step = (size_t)p.tokens * a.heads;
-        float2 e[2];
-        float m = -INFINITY;
+    float m = fmaxf(e[0].x, e[1].x);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float w[2], l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            e[k] = lane + 32 * k < a.splits ? a.ml[at + (lane + 32 * k) * step] : make_float2(-INFINITY, 0.0f);
-            m = fmaxf(m, e[k].x);
+    for (int k = 0; k < 2; ++k) {
+        w[k] = e[k].x == -INFINITY ? 0.0f : ex2f((e[k].x - m) * a.scale2);
+        if (w[k] != 0.0f) l = __fmaf_rn(w[k], e[k].y, l);
+    }
+    // NaN statistics (a NaN score) have m_i = -inf or a NaN sum: the sum carries them
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (e[k].y != e[k].y) l = e[k].y;
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float f = l > 0.0f || l != l ? a.vscale / l : 0.0f;
+    const int hd = p.head_dim, d = 4 * lane;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i0 = 0; i0 < a.splits; i0 += 4) {
+        float4 x[4];
+        float wi[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + k;
+            wi[k] = __shfl_sync(0xffffffffu, i < 32 ? w[0] : w[1], i & 31);
+            // (an empty split left nothing to read)
+            x[k] = i < a.splits && wi[k] != 0.0f && d < hd
+                       ? *reinterpret_cast<const float4*>(a.part + (at + i * step) * hd + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float w[2], l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            w[k] = e[k].x == -INFINITY ? 0.0f : ex2f((e[k].x - m) * a.scale2);
-            if (w[k] != 0.0f) l = __fmaf_rn(w[k], e[k].y, l);
-        }
-        // NaN statistics (a NaN score) have m_i = -inf or a NaN sum: the sum carries them
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (e[k].y != e[k].y) l = e[k].y;
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const float f = l > 0.0f || l != l ? a.vscale / l : 0.0f;
-        for (int d0 = 0; d0 < hd; d0 += 128) {
-            const int d = d0 + 4 * lane;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int i = 0; i < a.splits; ++i) {
-                const float wi = __shfl_sync(0xffffffffu, i < 32 ? w[0] : w[1], i & 31);
-                if (wi == 0.0f || d >= hd) continue;     // an empty split left nothing to read
-                const float4 x = *reinterpret_cast<const float4*>(a.part + (at + i * step) * hd + d);
-                v.x = __fmaf_rn(wi, x.x, v.x);
-                v.y = __fmaf_rn(wi, x.y, v.y);
-                v.z = __fmaf_rn(wi, x.z, v.z);
-                v.w = __fmaf_rn(wi, x.w, v.w);
-            }
-            if (d < hd)
-                store4_as(a.out, a.out_type, (long long)tok * a.out_stride + (long long)head * hd + d,
-                          make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+        for (int k = 0; k < 4; ++k) {
+            v.x = __fmaf_rn(wi[k], x[k].x, v.x);
+            v.y = __fmaf_rn(wi[k], x[k].y, v.y);
+            v.z = __fmaf_rn(wi[k], x[k].z, v.z);
+            v.w = __fmaf_rn(wi[k], x[k].w, v.w);
         }
     }
+    if (d < hd)
+        store4_as(a.out, a.out_type, (long long)tok * a.out_stride + (long long)head * hd + d,
+                  make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
 }
 
 // ---------------------------------------------------------------------------
@@ -400,8 +405,8 @@ struct AttnPlan {
 // Splits of the few-row kernel (a power of two: a cluster's blocks lie in one GPC): as
 // many as the GPU holds at once, of two tiles of 64 positions or more; twice that or
 // more of long sequences, whose ragged lengths then even out (12 x 40k positions: 1, 2, 4,
-// 8 splits 457, 274, 278, 244 us).  Of the many-row kernel: a block on every SM, of
-// eight tiles of 128 or more; they leave partial results in the work buffer, for a second
+// 8 splits 457, 274, 278, 244 us).  Of the many-row kernel: what
+// one block on each SM allows, of eight tiles of 128 or more; they leave partial results in the work buffer, for a second
 // kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
@@ -413,7 +418,7 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
     const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
     const int tiles = (b->max_len + tile - 1) / tile;
     if (pl.chunk) {
-        pl.splits = (int)std::max(1LL, std::min({(sms + units - 1) / units, (long long)tiles / 8, (long long)kPagedMaxSplits}));
+        pl.splits = (int)std::max(1LL, std::min({sms / units, (long long)tiles / 8, (long long)kPagedMaxSplits}));
     } else {
         const int es = p->format == VC4_KV_Q8 ? 1 : 2;
         const long long fit = (long long)sms * split_blocks(es, p->head_dim, pl.wr);
@@ -556,7 +561,7 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
         default: ok = pl.chunk ? launch_paged_chunk_f16(a, st) : launch_paged_split_f16(a, pl.wr, st); break;
     }
     if (!ok) return fail(VC4_ECUDA, "paged_attention: no TMA descriptor for this pool");
-    if (pl.bytes) launch_pdl_block(k_paged_join, dim3((unsigned)b->tokens), 128, 0, st, a);
+    if (pl.bytes) launch_pdl_block(k_paged_join, dim3((unsigned)(((long long)b->tokens * heads + 7) / 8)), 256, 0, st, a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return fail(VC4_ECUDA, std::string("paged_attention: ") + cudaGetErrorString(e));
     return VC4_OK;

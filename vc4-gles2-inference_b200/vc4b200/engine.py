@@ -188,7 +188,7 @@ class GPU:
         """Which drafted tokens stand and the sampled token behind them
         (vc4_verify_draft).  Arrays are raw device pointers as ints, 0 where an
         optional one is absent; logits_type "f32", "bf16", "f16" or "q16"."""
-        _check(lib().vc4_verify_draft(self._h, seqs, rows, vocab, cu, fed, logits, _dtype(logits_type), logits_stride,
+        _check(lib().vc4_verify_draft(self._h, seqs, rows, vocab, cu, fed, logits, _DTYPE[logits_type], logits_stride,
                                       probs, probs_stride, temperature, u, u_sample, next_tokens, accepted, prob,
                                       status, work, work_bytes, _stream(stream)))
 
@@ -204,11 +204,14 @@ class GPU:
             pass
 
 
-def _dtype(name: str) -> int:
-    try:
-        return DTYPES[name]
-    except KeyError:
-        raise EngineError("unknown element type %r (one of %s)" % (name, ", ".join(DTYPES))) from None
+class _Names(dict):
+    """Names of constants; an unknown one raises EngineError."""
+
+    def __missing__(self, name):
+        raise EngineError("unknown element type %r (one of %s)" % (name, ", ".join(self)))
+
+
+_DTYPE = _Names(DTYPES)
 
 
 def _stream(stream):
@@ -246,8 +249,8 @@ class PagedKV:
                rope_half: bool = True, qkv_stride: int = 0, q_stride: int = 0, stream: int = None):
         """Write the new tokens' K and V, normalised and rotated, into their
         pages and the rotated q rows to `q` (vc4_paged_append)."""
-        _check(lib().vc4_paged_append(self.gpu._h, self._p, batch._p, qkv, _dtype(qkv_type), qkv_stride, heads, q_norm,
-                                      k_norm, eps, cos, sin, rope_len, 1 if rope_half else 0, q, _dtype(q_type),
+        _check(lib().vc4_paged_append(self.gpu._h, self._p, batch._p, qkv, _DTYPE[qkv_type], qkv_stride, heads, q_norm,
+                                      k_norm, eps, cos, sin, rope_len, 1 if rope_half else 0, q, _DTYPE[q_type],
                                       q_stride, _stream(stream)))
 
     def attend_bytes(self, batch: PagedBatch, heads: int) -> int:
@@ -260,8 +263,8 @@ class PagedKV:
                work_bytes: int = 0, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, stream: int = None):
         """Attention of the new tokens over their sequences' pages
         (vc4_paged_attention)."""
-        _check(lib().vc4_paged_attention(self.gpu._h, self._p, batch._p, q, _dtype(q_type), q_stride, heads, scale, out,
-                                         _dtype(out_type), out_stride, work, work_bytes, _stream(stream)))
+        _check(lib().vc4_paged_attention(self.gpu._h, self._p, batch._p, q, _DTYPE[q_type], q_stride, heads, scale, out,
+                                         _DTYPE[out_type], out_stride, work, work_bytes, _stream(stream)))
 
 
 class Model:
