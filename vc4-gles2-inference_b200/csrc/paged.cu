@@ -400,18 +400,21 @@ struct AttnPlan {
 
 // Up to 64 rows (new tokens x query heads of a KV head) of a sequence go to the
 // few-row kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
-// the many-row kernel, 256 a block.  q16 pages with an f16 or float output stay
+// the many-row kernel, 256 a block; of large heads from 33 rows, where every SM has a
+// block (32 x 16 tokens over 4000 bf16 positions, 32/8 heads of 128: 133 us in blocks of
+// 64 rows, 111 in the many-row kernel; 61 x 5 over 2000, 16/2 of 64: 29 and 35).  q16 pages with an f16 or float output stay
 // with the few-row kernel, which holds a level in two operands.
-// Splits of the few-row kernel (a power of two: a cluster's blocks lie in one GPC): as
-// many as the GPU holds at once, of two tiles of 64 positions or more; twice that or
-// more of long sequences, whose ragged lengths then even out (12 x 40k positions: 1, 2, 4,
-// 8 splits 457, 274, 278, 244 us).  Of the many-row kernel: what
+// Splits of the few-row kernel: as many as the GPU holds at once, of three tiles of 64
+// positions or more; a whole cluster of eight for long sequences that do not fill the GPU
+// a whole number of times, whose ragged lengths then even out (12 x 40k positions: 1, 2,
+// 3, 4, 8 splits 457, 274, 283, 278, 244 us).  Of the many-row kernel: what
 // one block on each SM allows, of eight tiles of 128 or more; they leave partial results in the work buffer, for a second
 // kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
     const long long rows = (long long)b->max_new * (heads / p->kv_heads);
-    pl.chunk = rows > 64 && !(p->format == VC4_KV_Q16 && out_type != VC4_BF16);
+    const bool many = rows > 64 || (rows > 32 && p->head_dim > 96 && (long long)b->seqs * p->kv_heads >= sms);
+    pl.chunk = many && !(p->format == VC4_KV_Q16 && out_type != VC4_BF16);
     pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     const int per = pl.chunk ? 256 : 16 * pl.wr, tile = pl.chunk ? 128 : 64;
     pl.row_tiles = (int)((rows + per - 1) / per);
@@ -423,8 +426,8 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
         const int es = p->format == VC4_KV_Q8 ? 1 : 2;
         const long long fit = (long long)sms * split_blocks(es, p->head_dim, pl.wr);
         pl.splits = 1;
-        while (pl.splits < kPagedMaxCluster && 2 * pl.splits * units <= fit && tiles >= 4 * pl.splits) pl.splits *= 2;
-        while (pl.splits < kPagedMaxCluster && pl.splits * units * 2 > fit && units < fit && tiles >= 128 * pl.splits) pl.splits *= 2;
+        pl.splits = (int)std::max(1LL, std::min({fit / units, (long long)tiles / 3, (long long)kPagedMaxCluster}));
+        if (units < fit && fit / units < kPagedMaxCluster && tiles >= 128 * pl.splits) pl.splits = kPagedMaxCluster;
     }
     if (pl.chunk && pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
     return pl;
