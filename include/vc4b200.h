@@ -321,7 +321,8 @@ VC4_API int vc4_read_buffer(vc4_session* s, int slot, int buf, int n, float* out
    code seen is left in *status where the batch has one (set it to 0 before): a
    page id outside the pool, a position outside the page table or the rotation
    tables, a length below the new tokens, a token id outside the vocabulary give
-   VC4_EINVAL, a row of logits without a finite value VC4_ERANGE. */
+   VC4_EINVAL, a NaN logit or a row of logits without a finite value VC4_ERANGE; a
+   kernel's bounded wait that ran out VC4_ECUDA (the call's outputs are void). */
 
 /* Element types of activations.  VC4_Q16I: int32 values on the q16 grid (1/256),
    the form of this engine's own logits. */
@@ -384,7 +385,9 @@ VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_bat
    VC4_F16 and, for bf16 and f16 pages, the pages' own; out_type any of VC4_F32,
    VC4_BF16, VC4_F16.  Products run on the tensor cores (bf16 pages: bf16, others:
    f16; a bf16 q beyond +-65504 is taken as that), sums and softmax statistics in
-   float.  A row that sees no position is zero.  work: work_bytes of
+   float.  A row that sees no position is zero; positions it does not see (later new
+   tokens, rows of a page behind the length) may hold anything.  A row that sees an
+   infinite or NaN V of a later new token's position is NaN as a whole.  work: work_bytes of
    vc4_paged_attention_bytes for the same pages, heads and batch bounds (NULL when
    that is 0), free again when the call's work is done. */
 VC4_API int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* q, int q_type,
@@ -397,7 +400,7 @@ VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_
    target model rows cu[s] .. cu[s+1]-1: its last token, then its drafts; `fed`
    holds those ids, `logits` (rows logits_stride elements apart; 0: vocab) what
    each row predicts, p = softmax(logits / temperature) (temperature 0: the first
-   maximum).  The draft after row i of sequence s (the next fed id, x) is accepted
+   maximum; else 1e-5 or more).  The draft after row i of sequence s (the next fed id, x) is accepted
    while u[row] * d(x) < p(x), d being the draft's row of draft_probs (one row for
    each draft of the batch in order, probs_stride apart; 0: vocab), or one at x and
    zero elsewhere when draft_probs is NULL.  The first refused row is sampled from max(p - d, 0) normalised (from p

@@ -358,6 +358,33 @@ def test_attend_infinite_and_nan_values_reach_only_rows_that_see_them():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim,new,past", [(2, 1, 64, 5, 40), (8, 2, 128, 9, 300), (4, 4, 96, 7, 5000), (4, 1, 128, 100, 60),
+                                                   (2, 2, 64, 300, 200), (8, 1, 80, 90, 3000)])
+def test_attend_wild_values_of_later_tokens_stay_there(fmt, heads, kv, dim, new, past):
+    """A new token whose K and V are infinite or NaN: the rows before it come out as
+    without it, it and those after it are not finite."""
+    at = new * 2 // 3
+    cache = Cache([past + new, 33], [new, 1], fmt, 16, kv, dim)
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(new + 1, heads * dim, generator=g).to(TORCH[fmt]).cuda()
+    clean, _ = _attend(cache, heads, fmt, "f32", q)
+    pos = past + at
+    pg = int(cache.host_table[0, pos // 16])
+    for k_value, v_value in ((None, float("inf")), (None, float("nan")), (float("nan"), float("-inf"))):
+        pool = cache.pool.clone()
+        cache.pool[pg, 1, kv - 1, pos % 16, dim - 1] = v_value
+        cache.pool[pg, 1, kv - 1, pos % 16, 0] = v_value
+        if k_value is not None:
+            cache.pool[pg, 0, :, pos % 16] = k_value
+        out, _ = _attend(cache, heads, fmt, "f32", q)
+        assert torch.equal(out[:at], clean[:at]) and torch.equal(out[new:], clean[new:])
+        mine = out[at:new].view(new - at, heads, dim)[:, -1]     # the last query head reads the last KV head
+        assert not bool(torch.isfinite(mine[:, [0, dim - 1]]).any())
+        cache.pool.copy_(pool)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt,kind", [("q8", "bf16"), ("bf16", "bf16")])
 def test_attend_same_bits_twice_and_on_another_stream(fmt, kind):
     cache = Cache([3000, 77], [2, 2], fmt, 32, 2, 128)

@@ -139,7 +139,7 @@ class _Host(vc4b200.GPU):
 
 @pytest.mark.parametrize("over,words", [
     (dict(seqs=0), "seqs"), (dict(vocab=0), "vocab"), (dict(rows=-1), "not negative"), (dict(rows=2 ** 31 - 1, vocab=100000), "too many"), (dict(seqs=2 ** 25), "too many"),
-    (dict(temperature=-1.0), "temperature"), (dict(temperature=math.nan), "temperature"), (dict(temperature=math.inf), "temperature"),
+    (dict(temperature=-1.0), "temperature"), (dict(temperature=math.nan), "temperature"), (dict(temperature=math.inf), "temperature"), (dict(temperature=1e-6), "temperature"),
     (dict(cu=0), "null"), (dict(fed=0), "null"), (dict(logits=0), "null"), (dict(u=0), "null"), (dict(u_sample=0), "null"),
     (dict(next_tokens=0), "null"), (dict(accepted=0), "null"), (dict(logits=66), "aligned"), (dict(probs=66), "aligned"),
     (dict(logits_stride=99), "stride"), (dict(probs_stride=99), "stride"), (dict(work=0), "work buffer"), (dict(work=72), "work buffer"),

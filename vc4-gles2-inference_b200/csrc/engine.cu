@@ -721,8 +721,8 @@ int vc4_step_draft(vc4_session* s, int slot, const int* tokens, int n, int pos0,
     if (!s) return fail(VC4_EINVAL, "step_draft: session is null");
     if (n <= 0 || n > s->slots) return fail(VC4_EINVAL, "step_draft: the fed tokens must be 1 .. slots");
     if (!tokens || !next || !accepted || (n > 1 && !u)) return fail(VC4_EINVAL, "step_draft: a required array is null");
-    if (!(temperature >= 0.0f) || !(temperature < INFINITY))
-        return fail(VC4_EINVAL, "step_draft: temperature must not be negative");
+    if (!(temperature == 0.0f || temperature >= 1e-5f) || !(temperature < INFINITY))
+        return fail(VC4_EINVAL, "step_draft: temperature must be 0 or at least 1e-5");
     if (int e = check_slot_pos(s, slot, pos0)) return e;
     if (n > s->st.seq - pos0) return fail(VC4_EINVAL, "step_draft: the drafts run past the sequence length");
     const DModel& m = s->m->d;

@@ -83,6 +83,33 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
+// Whether one of the eight 16-bit floats is infinite or NaN.
+template <int FMT>
+__device__ __forceinline__ bool any_wild(const uint4 v) {
+    constexpr unsigned top = FMT == P_BF16 ? 0x7F807F80u : 0x7C007C00u;   // all exponent bits
+    auto wild = [](unsigned w) { return (w & (top & 0xFFFFu)) == (top & 0xFFFFu) || (w & (top & 0xFFFF0000u)) == (top & 0xFFFF0000u); };
+    return wild(v.x) || wild(v.y) || wild(v.z) || wild(v.w);
+}
+// The same values with 0 for those.
+template <int FMT>
+__device__ __forceinline__ uint4 tamed(uint4 v) {
+    constexpr unsigned top = FMT == P_BF16 ? 0x7F807F80u : 0x7C007C00u;
+    auto tame = [](unsigned w) {
+        if ((w & (top & 0xFFFFu)) == (top & 0xFFFFu)) w &= 0xFFFF0000u;
+        if ((w & (top & 0xFFFF0000u)) == (top & 0xFFFF0000u)) w &= 0xFFFFu;
+        return w;
+    };
+    return make_uint4(tame(v.x), tame(v.y), tame(v.z), tame(v.w));
+}
+__device__ __forceinline__ uint4 ld_shared16(unsigned addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void st_shared16(unsigned addr, const uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 template <int FMT> struct PagedBytes { static constexpr int v = FMT == P_Q8 ? 1 : 2; };
 
 // Two 16-bit operands in one register.

@@ -589,7 +589,9 @@ extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const
     if (!logits_stride) logits_stride = vocab;
     if (!probs_stride) probs_stride = vocab;
     if (logits_stride < vocab || probs_stride < vocab) return refuse("a stride is below the vocabulary");
-    if (!(temperature >= 0.0f) || !(temperature < INFINITY)) return refuse("temperature must not be negative");
+    // (below this the logits' products with 1/T would leave double's whole numbers)
+    if (!(temperature == 0.0f || temperature >= 1e-5f) || !(temperature < INFINITY))
+        return refuse("temperature must be 0 or at least 1e-5");
     if (!cu || !fed || !logits || !u || !u_sample || !next || !accepted) return refuse("a required array is null");
     const int es = logits_type == VC4_BF16 || logits_type == VC4_F16 ? 2 : 4;
     if ((uintptr_t)logits % es || (uintptr_t)draft_probs % 4) return refuse("an array is not aligned to its elements");
