@@ -385,6 +385,40 @@ def test_attend_wild_values_of_later_tokens_stay_there(fmt, heads, kv, dim, new,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,new", [("q8", 2), ("q8", 150), ("bf16", 2), ("bf16", 150), ("q16", 150)])
+def test_pool_beyond_32_bits(fmt, new):
+    """Pages whose bytes and values lie past 2^32: append and attention find them."""
+    kv, dim, page, heads = 4, 64, 64, 8
+    cache = Cache([300 + new, 70 + new], [new, new], fmt, page, kv, dim)
+    small_pool, small_table, per = cache.pool, cache.host_table, 2 * kv * page * dim
+    shift = (1 << 32) // per + 7
+    big = torch.empty((shift + cache.pages) * per, dtype=POOL[fmt], device="cuda")
+    big = big.view(-1, 2, kv, page, dim)
+    big[shift:] = small_pool
+    cache.table += shift * (cache.table >= 0).int()
+    t, kw = _append_case(cache, heads, "bf16", _kind(fmt), True, True)
+    gpu = vc4b200.GPU(0)
+    handle, batch = cache.handles(vc4b200, gpu)
+    handle = vc4b200.PagedKV(gpu, big.data_ptr(), fmt, big.shape[0], page, kv, dim)
+    out = torch.zeros(2 * new, heads * dim, device="cuda")
+    need = handle.attend_bytes(batch, heads)
+    work = torch.empty(max(16, need), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    handle.append(batch, t["qkv"].data_ptr(), "bf16", heads, t["q"].data_ptr(), _kind(fmt), **kw)
+    handle.attend(batch, t["q"].data_ptr(), _kind(fmt), heads, out.data_ptr(), "f32", work.data_ptr(), need)
+    gpu.sync()
+    assert int(cache.status) == 0
+    cache.pool = big[shift:]
+    q, k, v, off = _append_ref(cache, t, heads, True, True, True)
+    row, pos = new - 1, cache.length[0] - 1
+    have = decode(cache.pool, fmt)[int(small_table[0, pos // page]), 0, :, pos % page]
+    step = 0.5 / GRID[fmt] if fmt in GRID else half_step(fmt) * float(k[row].abs().max())
+    assert bool(((have - k[row].clamp(-16, 16)).abs() <= step * 1.01 + off[row, heads: heads + kv] + 1e-6).all())
+    want, mass, top = attention(cache, t["q"], heads)
+    assert bool(((out.double().view_as(want) - want).abs() <= attention_bound(fmt, "f32", want, mass, top, dim)).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt,kind", [("q8", "bf16"), ("bf16", "bf16")])
 def test_attend_same_bits_twice_and_on_another_stream(fmt, kind):
     cache = Cache([3000, 77], [2, 2], fmt, 32, 2, 128)

@@ -186,6 +186,66 @@ def test_verify_strides_and_alignment(kind, pad, shift):
 
 
 @pytest.mark.gpu
+def test_verify_rows_beyond_32_bits():
+    """Rows 2^27 values apart: the last ones start past 2^32."""
+    vocab, stride, counts = 700, 1 << 27, [20, 21]
+    logits, value, fed, _, u, us = make(counts, vocab, "bf16", False, 12)
+    want = reference(counts, fed, value, None, u, us, 0.9)
+    assert want[3]
+    buf = torch.empty(40 * stride + vocab, dtype=torch.bfloat16, device="cuda")
+    torch.as_strided(buf, (41, vocab), (stride, 1)).copy_(logits)
+    gpu = vc4b200.GPU(0)
+    ints = lambda x: torch.as_tensor(np.asarray(x), dtype=torch.int32).cuda()  # noqa: E731
+    cu, f, uu, uz = ints([0, 20, 41]), ints(fed), torch.from_numpy(u).cuda(), torch.from_numpy(us).cuda()
+    nxt, acc = ints(np.zeros(41)), ints(np.zeros(2))
+    need = gpu.verify_bytes(2, 41, vocab)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    gpu.verify_draft(2, 41, vocab, cu.data_ptr(), f.data_ptr(), buf.data_ptr(), "bf16", 0.9, uu.data_ptr(), uz.data_ptr(),
+                     nxt.data_ptr(), acc.data_ptr(), 0, work.data_ptr(), need, logits_stride=stride)
+    gpu.sync()
+    assert np.array_equal(nxt.cpu().numpy(), want[0]) and np.array_equal(acc.cpu().numpy(), want[1])
+
+
+@pytest.mark.gpu
+def test_verify_captured_and_on_two_streams():
+    """A captured call follows its arrays; two calls with buffers of their own overlap."""
+    gpu, runs = vc4b200.GPU(0), []
+    for seed in (1, 2):
+        counts = [4, 6]
+        logits, value, fed, probs, u, us = make(counts, 3001, "f32", True, seed)
+        t = {"cu": torch.tensor([0, 4, 10], dtype=torch.int32).cuda(), "fed": torch.from_numpy(fed).int().cuda(),
+             "logits": logits.cuda(), "probs": probs.cuda(), "u": torch.from_numpy(u).cuda(), "us": torch.from_numpy(us).cuda(),
+             "next": torch.zeros(10, dtype=torch.int32).cuda(), "acc": torch.zeros(2, dtype=torch.int32).cuda()}
+        need = gpu.verify_bytes(2, 10, 3001)
+        t["work"] = torch.empty(need, dtype=torch.uint8, device="cuda")
+
+        def step(t=t, need=need):
+            gpu.verify_draft(2, 10, 3001, t["cu"].data_ptr(), t["fed"].data_ptr(), t["logits"].data_ptr(), "f32", 1.0,
+                             t["u"].data_ptr(), t["us"].data_ptr(), t["next"].data_ptr(), t["acc"].data_ptr(), 0,
+                             t["work"].data_ptr(), need, probs=t["probs"].data_ptr(),
+                             stream=torch.cuda.current_stream().cuda_stream)
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        runs.append((graph, t, counts, value, fed, probs, u, us))
+    for change in (False, True):
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for (graph, t, *_), st in zip(runs, streams):
+            if change:
+                t["us"].copy_(1 - t["us"])
+                torch.cuda.synchronize()
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, t, counts, value, fed, probs, u, us in runs:
+            want = reference(counts, fed, value, probs.numpy(), u, t["us"].cpu().numpy(), 1.0)
+            assert want[3] and np.array_equal(t["next"].cpu().numpy(), want[0])
+
+
+@pytest.mark.gpu
 def test_verify_many_drafts_and_many_sequences():
     check([70, 33, 32, 31], 200, "f32", True, 1.3, seed=2)     # the walk takes 32 rows at a time
     check([2] * 500, 300, "bf16", True, 1.0, seed=3)
