@@ -412,7 +412,7 @@ VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_
    or VC4_Q16I.  `rows` bounds cu[seqs].  NaN logits count as -inf. */
 VC4_API int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const int* cu, const int* fed,
                              const void* logits, int logits_type, long long logits_stride, const float* draft_probs,
-                             long long probs_stride, float temperature, const float* u, const float* u_sample,
+                             long long probs_stride, double temperature, const float* u, const float* u_sample,
                              int* next, int* accepted, float* prob, int* status, void* work, size_t work_bytes,
                              void* stream);
 VC4_API int vc4_verify_draft_bytes(int seqs, int rows, int vocab, size_t* bytes);
@@ -425,7 +425,7 @@ VC4_API int vc4_verify_draft_bytes(int seqs, int rows, int vocab, size_t* bytes)
    positions pos0 .. pos0 + *accepted are decoded, the rows behind them are
    overwritten by the next step.  n is at most the session's slots.  Synchronous. */
 VC4_API int vc4_step_draft(vc4_session* s, int slot, const int* tokens, int n, int pos0, const float* draft_probs,
-                           float temperature, const float* u, float u_sample, int* next, int* accepted, float* prob);
+                           double temperature, const float* u, float u_sample, int* next, int* accepted, float* prob);
 
 /* draws()/syncs() (gpu.h:44-48): kernels launched and host syncs so far. */
 VC4_API int vc4_counters(const vc4_session* s, long long* launches, long long* syncs);

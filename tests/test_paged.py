@@ -184,6 +184,36 @@ def test_append(fmt, heads, kv, dim, page, kind, out_kind, norm, half, rope):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["q8", "q16"])
+@pytest.mark.parametrize("kind,half", [("f32", True), ("bf16", False), ("f16", True)])
+def test_append_levels_are_the_slot_caches_arithmetic(fmt, kind, half):
+    """Every level and q value of many tokens: the float operations one by one
+    (squares in double), as the slot cache's kernels round them."""
+    heads, kv, dim, n = 16, 8, 96, 4000
+    cache = Cache([n], [n], fmt, 32, kv, dim)
+    t, kw = _append_case(cache, heads, kind, "f32", True, half)
+    gpu = vc4b200.GPU(0)
+    handle, batch = cache.handles(vc4b200, gpu)
+    torch.cuda.synchronize()
+    handle.append(batch, t["qkv"].data_ptr(), kind, heads, t["q"].data_ptr(), "f32", **kw)
+    gpu.sync()
+    x = t["qkv"].float().view(n, heads + 2 * kv, dim)
+    y = x[:, : heads + kv]
+    mean = y.double().square().sum(-1, keepdim=True).float() / torch.full((), float(dim), device="cuda")
+    y = torch.cat([t["qn"].expand(heads, dim), t["kn"].expand(kv, dim)]) * ((1 / (mean + 1e-6).sqrt()) * y)
+    c, s = t["cos"][:n, None], t["sin"][:n, None]
+    a, b = (y[..., : dim // 2], y[..., dim // 2:]) if half else (y[..., 0::2], y[..., 1::2])
+    u, v = a * c - b * s, a * s + b * c
+    y = torch.cat([u, v], -1) if half else torch.stack([u, v], -1).flatten(-2)
+    assert torch.equal(t["q"].view(n, heads, dim), y[:, :heads])
+    want = torch.stack([y[:, heads:], x[:, heads + kv:]], 1)
+    grid, low, high = (16, -128, 127) if fmt == "q8" else (2048, -32768, 32767)
+    want = (want * grid + 0.5).floor().clamp(low, high) / grid
+    have = cache.rows_of(0).permute(2, 0, 1, 3).float()
+    assert torch.equal(have, want)
+
+
+@pytest.mark.gpu
 def test_append_codec_borders_and_rails():
     """The codec's ties, rails and infinities, value by value, as the slot cache's own encoder gives them."""
     dim = 16

@@ -717,11 +717,11 @@ int vc4_prefill_logits(vc4_session* s, int slot, const int* tokens, int n, int p
 // logits bit for bit, so the drafts cost one pass; models and lengths outside
 // the many-sequence kernels step position by position into a logits buffer.
 int vc4_step_draft(vc4_session* s, int slot, const int* tokens, int n, int pos0, const float* draft_probs,
-                   float temperature, const float* u, float u_sample, int* next, int* accepted, float* prob) {
+                   double temperature, const float* u, float u_sample, int* next, int* accepted, float* prob) {
     if (!s) return fail(VC4_EINVAL, "step_draft: session is null");
     if (n <= 0 || n > s->slots) return fail(VC4_EINVAL, "step_draft: the fed tokens must be 1 .. slots");
     if (!tokens || !next || !accepted || (n > 1 && !u)) return fail(VC4_EINVAL, "step_draft: a required array is null");
-    if (!(temperature == 0.0f || temperature >= 1e-5f) || !(temperature < INFINITY))
+    if (!(temperature == 0.0 || temperature >= 1e-5) || !(temperature < INFINITY))
         return fail(VC4_EINVAL, "step_draft: temperature must be 0 or at least 1e-5");
     if (int e = check_slot_pos(s, slot, pos0)) return e;
     if (n > s->st.seq - pos0) return fail(VC4_EINVAL, "step_draft: the drafts run past the sequence length");

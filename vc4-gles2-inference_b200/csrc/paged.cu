@@ -100,7 +100,7 @@ __device__ __forceinline__ void store_cache4(uint8_t* row, int i, float4 v) {
 // one vector's and takes its root.
 // The float operations are the slot cache's (k_attn): squares summed in double,
 // 1/sqrt(ss/hd + eps), w*(r*x), the rotation's products and sums rounded one by one, the
-// codec's floor(x*grid + 1/2).  Packed products and sums round like single ones.
+// codec's floor(x*grid + 1/2).  (Packed products round like single ones.)
 template <int TIN, int FMT, int LPV>
 __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
     constexpr int N = kAppendVecs, NG = 32 / LPV;   // groups of a warp
@@ -220,33 +220,31 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
             if (a.cos) {
                 const float4 c = *reinterpret_cast<const float4*>(a.cos + (size_t)pos * half + 4 * sub);
                 const float4 s = *reinterpret_cast<const float4*>(a.sin + (size_t)pos * half + 4 * sub);
-                const unsigned long long c0 = pack2(c.x, c.y), c1 = pack2(c.z, c.w), s0 = pack2(s.x, s.y), s1 = pack2(s.z, s.w);
-                const unsigned long long m0 = pack2(-s.x, -s.y), m1 = pack2(-s.z, -s.w);
-                auto turn = [](unsigned long long& u, unsigned long long& v, unsigned long long cc, unsigned long long sn,
-                               unsigned long long neg) {
-                    const unsigned long long y = add2(mul2(u, cc), mul2(v, neg));   // a c - b s, rounded as that
-                    v = add2(mul2(u, sn), mul2(v, cc));
+                // (single operations: a packed product and sum may come out as one rounding)
+                auto turn = [](float& u, float& v, float cc, float ss) {
+                    const float y = __fsub_rn(__fmul_rn(u, cc), __fmul_rn(v, ss));
+                    v = __fadd_rn(__fmul_rn(u, ss), __fmul_rn(v, cc));
                     u = y;
                 };
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
                     if (vec0 + k >= turned) continue;
+                    float4 f0 = as_float4(x[k][0]), f1 = as_float4(x[k][1]);
                     if (a.half) {
-                        turn(x[k][0][0], x[k][1][0], c0, s0, m0);
-                        turn(x[k][0][1], x[k][1][1], c1, s1, m1);
-                    } else {                                  // neighbours: apart, turned, together again
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float4 f = as_float4(x[k][h]);
-                            unsigned long long u = pack2(f.x, f.z), v = pack2(f.y, f.w);
-                            turn(u, v, h ? c1 : c0, h ? s1 : s0, h ? m1 : m0);
-                            float u0, u1, v0, v1;
-                            unpack2(u, u0, u1);
-                            unpack2(v, v0, v1);
-                            x[k][h][0] = pack2(u0, v0);
-                            x[k][h][1] = pack2(u1, v1);
-                        }
+                        turn(f0.x, f1.x, c.x, s.x);
+                        turn(f0.y, f1.y, c.y, s.y);
+                        turn(f0.z, f1.z, c.z, s.z);
+                        turn(f0.w, f1.w, c.w, s.w);
+                    } else {
+                        turn(f0.x, f0.y, c.x, s.x);
+                        turn(f0.z, f0.w, c.y, s.y);
+                        turn(f1.x, f1.y, c.z, s.z);
+                        turn(f1.z, f1.w, c.w, s.w);
                     }
+                    x[k][0][0] = pack2(f0.x, f0.y);
+                    x[k][0][1] = pack2(f0.z, f0.w);
+                    x[k][1][0] = pack2(f1.x, f1.y);
+                    x[k][1][1] = pack2(f1.z, f1.w);
                 }
             }
             const long long qrow = (long long)(tok0 + t) * a.q_stride;

@@ -579,7 +579,7 @@ extern "C" int vc4_verify_draft_bytes(int seqs, int rows, int vocab, size_t* byt
 
 extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const int* cu, const int* fed,
                                 const void* logits, int logits_type, long long logits_stride, const float* draft_probs,
-                                long long probs_stride, float temperature, const float* u, const float* u_sample,
+                                long long probs_stride, double temperature, const float* u, const float* u_sample,
                                 int* next, int* accepted, float* prob, int* status, void* work, size_t work_bytes,
                                 void* stream) {
     auto refuse = [](const std::string& m) { return vfail(VC4_EINVAL, "verify_draft: " + m); };
@@ -590,7 +590,7 @@ extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const
     if (!probs_stride) probs_stride = vocab;
     if (logits_stride < vocab || probs_stride < vocab) return refuse("a stride is below the vocabulary");
     // (below this the logits' products with 1/T would leave double's whole numbers)
-    if (!(temperature == 0.0f || temperature >= 1e-5f) || !(temperature < INFINITY))
+    if (!(temperature == 0.0 || temperature >= 1e-5) || !(temperature < INFINITY))
         return refuse("temperature must be 0 or at least 1e-5");
     if (!cu || !fed || !logits || !u || !u_sample || !next || !accepted) return refuse("a required array is null");
     const int es = logits_type == VC4_BF16 || logits_type == VC4_F16 ? 2 : 4;
@@ -611,7 +611,7 @@ extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const
     a.cu = cu; a.fed = fed; a.logits = logits; a.stride = logits_stride; a.probs_stride = probs_stride;
     a.probs = draft_probs; a.u = u; a.u_sample = u_sample; a.next = next; a.accepted = accepted; a.status = status;
     a.prob = prob; a.part = (VerifyPart*)work; a.chunks = verify_chunks(rows, vocab);
-    a.inv_t = temperature > 0.0f ? 1.0 / (double)temperature : 0.0;
+    a.inv_t = temperature > 0.0 ? 1.0 / temperature : 0.0;
     a.scale2 = (float)(1.4426950408889634 * a.inv_t);
     a.scale256 = 1.44269504088896340736 * 256 * a.inv_t;
     switch (logits_type) {

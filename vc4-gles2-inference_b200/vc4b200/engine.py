@@ -112,11 +112,11 @@ _PROTOS = {
                                       C.c_void_p]),
     "vc4_paged_attention_bytes": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_size_t)]),
     "vc4_verify_draft": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
-                                   C.c_longlong, C.c_void_p, C.c_longlong, C.c_float, C.c_void_p, C.c_void_p,
+                                   C.c_longlong, C.c_void_p, C.c_longlong, C.c_double, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                    C.c_void_p]),
     "vc4_verify_draft_bytes": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
-    "vc4_step_draft": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_float, C.c_void_p,
+    "vc4_step_draft": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_double, C.c_void_p,
                                  C.c_float, C.c_void_p, C.POINTER(C.c_int), C.c_void_p]),
     "vc4_counters": (C.c_int, [C.c_void_p, C.POINTER(C.c_longlong), C.POINTER(C.c_longlong)]),
     "vc4_launches_per_step": (C.c_int, [C.c_void_p, C.c_int]),
