@@ -320,8 +320,8 @@ VC4_API int vc4_read_buffer(vc4_session* s, int slot, int buf, int n, float* out
    checked by the kernels: a bad entry is skipped, never followed, and the largest
    code seen is left in *status where the batch has one (set it to 0 before): a
    page id outside the pool, a position outside the page table or the rotation
-   tables, a length below the new tokens, a token id outside the vocabulary give
-   VC4_EINVAL, a NaN logit or a row of logits without a finite value VC4_ERANGE; a
+   tables, a length below the new tokens, offsets that run backwards or past the
+   batch's rows, a token id outside the vocabulary give VC4_EINVAL, a NaN logit or a row of logits without a finite value VC4_ERANGE; a
    kernel's bounded wait that ran out VC4_ECUDA (the call's outputs are void). */
 
 /* Element types of activations.  VC4_Q16I: int32 values on the q16 grid (1/256),
@@ -341,7 +341,7 @@ VC4_API int vc4_read_buffer(vc4_session* s, int slot, int buf, int n, float* out
 
 /* A pool of pages: [pages][2: K, V][kv_heads][page_len][head_dim], packed, its
    address a multiple of 16.  page_len: 16, 32, 64, 128 or 256; head_dim: a
-   multiple of 16, at most 128. */
+   multiple of 16, at most 128; at most 2^31 - 1 rows of head_dim values. */
 typedef struct {
     void* data;
     int format, pages, page_len, kv_heads, head_dim;
@@ -354,7 +354,8 @@ typedef struct {
    sequence may have no new token.  `tokens` bounds cu[seqs] (rows of it behind
    the last sequence are left as they were), max_new and max_len bound the new
    tokens and the length of one sequence: they choose the launch, so a captured
-   call holds for every content of the arrays within them. */
+   call holds for every content of the arrays within them.  table_stride x page_len
+   is at most 2^30. */
 typedef struct {
     int seqs, tokens, max_new, max_len, table_stride;
     const int* cu;       /* seqs + 1 */
@@ -372,7 +373,8 @@ typedef struct {
    the sequence's page, the rotated q to q ([heads][head_dim], q_stride apart).
    The operations and their order are the slot cache's, so the page bytes of the
    q8 / q16 formats are those vc4_kv_read_rows gives.  qkv_type and q_type:
-   VC4_F32, VC4_BF16 or VC4_F16.  Two sequences must not append into one page.
+   VC4_F32, VC4_BF16 or VC4_F16.  Two sequences must not append into one page, and
+   q must not overlap qkv.
    Addresses are multiples of 16, strides of 8 elements. */
 VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* qkv, int qkv_type,
                              long long qkv_stride, int heads, const float* q_norm, const float* k_norm, float eps,
@@ -387,9 +389,10 @@ VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_bat
    f16; a bf16 q beyond +-65504 is taken as that), sums and softmax statistics in
    float.  A row that sees no position is zero; positions it does not see (later new
    tokens, rows of a page behind the length) may hold anything.  A row that sees an
-   infinite or NaN V of a later new token's position is NaN as a whole.  work: work_bytes of
-   vc4_paged_attention_bytes for the same pages, heads and batch bounds (NULL when
-   that is 0), free again when the call's work is done. */
+   infinite or NaN V of a later new token's position is NaN as a whole.  out must not
+   overlap q.  work: work_bytes of vc4_paged_attention_bytes for the same pages,
+   heads and batch bounds (NULL when that is 0), free again when the call's work is
+   done. */
 VC4_API int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* q, int q_type,
                                 long long q_stride, int heads, float scale, void* out, int out_type,
                                 long long out_stride, void* work, size_t work_bytes, void* stream);
@@ -400,16 +403,18 @@ VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_
    target model rows cu[s] .. cu[s+1]-1: its last token, then its drafts; `fed`
    holds those ids, `logits` (rows logits_stride elements apart; 0: vocab) what
    each row predicts, p = softmax(logits / temperature) (temperature 0: the first
-   maximum; else 1e-5 or more).  The draft after row i of sequence s (the next fed id, x) is accepted
-   while u[row] * d(x) < p(x), d being the draft's row of draft_probs (one row for
-   each draft of the batch in order, probs_stride apart; 0: vocab), or one at x and
-   zero elsewhere when draft_probs is NULL.  The first refused row is sampled from max(p - d, 0) normalised (from p
-   where that is zero everywhere), and the last row, when all are accepted, from p:
+   maximum; else 1e-5 or more).  The draft after row i of sequence s (the next fed
+   id, x) is accepted while u[row] * d(x) < p(x), d being the draft's row of
+   draft_probs (one row for each draft of the batch in order, probs_stride apart; 0:
+   vocab), or one at x and zero elsewhere when draft_probs is NULL.  The first
+   refused row is sampled from max(p - d, 0) normalised (from p where that is zero
+   everywhere), and the last row, when all are accepted, from p:
    the first id whose cumulative sum exceeds u_sample[s] times the total, sums in
    double.  next: per row the accepted draft, then the sampled id, then -1;
    accepted (seqs): drafts accepted; prob (rows, or NULL): the target's probability
    of each id in next, 0 where that is -1.  logits_type: VC4_F32, VC4_BF16, VC4_F16
-   or VC4_Q16I.  `rows` bounds cu[seqs].  NaN logits count as -inf. */
+   or VC4_Q16I.  `rows` bounds cu[seqs].  NaN logits count as -inf.  An output that
+   overlaps an input or another output is refused. */
 VC4_API int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const int* cu, const int* fed,
                              const void* logits, int logits_type, long long logits_stride, const float* draft_probs,
                              long long probs_stride, double temperature, const float* u, const float* u_sample,

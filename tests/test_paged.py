@@ -40,7 +40,8 @@ def _refused(call, words):
 @pytest.mark.parametrize("over,words", [
     (dict(page_len=24), "page_len"), (dict(page_len=512), "page_len"), (dict(head_dim=72), "head_dim"),
     (dict(head_dim=144), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(pages=0), "positive"),
-    (dict(kv_heads=0), "positive"), (dict(data=0), "address"), (dict(data=264), "address")])
+    (dict(kv_heads=0), "positive"), (dict(data=0), "address"), (dict(data=264), "address"),
+    (dict(pages=2 ** 25, page_len=32), "2^31 - 1 rows"), (dict(pages=2 ** 31 - 1), "2^31 - 1 rows")])
 def test_pages_are_refused(over, words):
     _refused(lambda: _host_pages(**over).append(_host_batch(), 64, "f32", 4, 64, "bf16"), words)
     _refused(lambda: _host_pages(**over).attend(_host_batch(), 64, "bf16", 4, 64, "bf16"), words)
@@ -49,7 +50,7 @@ def test_pages_are_refused(over, words):
 @pytest.mark.parametrize("over,words", [
     (dict(seqs=0), "seqs"), (dict(tokens=-1), "not negative"), (dict(max_new=-1), "not negative"),
     (dict(table_stride=0), "table_stride"), (dict(max_len=33), "page table"), (dict(cu=0), "required"),
-    (dict(length=0), "required"), (dict(table=0), "required")])
+    (dict(length=0), "required"), (dict(table=0), "required"), (dict(table_stride=2 ** 26 + 1), "2^30 positions")])
 def test_batches_are_refused(over, words):
     _refused(lambda: _host_pages().append(_host_batch(**over), 64, "f32", 4, 64, "bf16"), words)
     _refused(lambda: _host_pages().attend(_host_batch(**over), 64, "bf16", 4, 64, "bf16"), words)
@@ -80,6 +81,8 @@ def test_append_refuses(fmt, args, more, words):
     ("q8", (64, "bf16", 4, 64, "bf16"), dict(out_stride=8), "stride"),
     ("q8", (64, "bf16", 4, 64, "bf16"), dict(scale=-0.5), "scale"),
     ("q8", (64, "bf16", 4, 64, "bf16"), dict(scale=math.nan), "scale"),
+    ("q8", (64, "bf16", 4, 64, "bf16"), dict(scale=1e-38), "float's range"),
+    ("bf16", (64, "bf16", 4, 64, "bf16"), dict(scale=3e38), "float's range"),
     ("q8", (64, "bf16", 4, 64, "bf16"), {}, "gpu is null")])
 def test_attend_refuses(fmt, args, more, words):
     _refused(lambda: _host_pages(fmt).attend(_host_batch(), *args, **more), words)
@@ -376,6 +379,20 @@ def test_attend_rows_that_see_nothing_are_zero(fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [2, 100])
+@pytest.mark.parametrize("cu", [(0, "all", "more"), (-1, "all", "all"), (0, "all", 1)])
+def test_attend_flags_bad_offsets(new, cu):
+    """Offsets past the batch's rows, below them or running backwards: flagged, nothing outside the rows touched."""
+    cache = Cache([300, 200], [new, new], "bf16", 16, 1, 64)
+    cache.cu.copy_(torch.tensor([{"all": new, "more": 2 * new + 1}.get(c, c) for c in cu], dtype=torch.int32))
+    if cu[2] == "all":
+        cache.cu[2] = 2 * new
+    q = torch.randn(cache.rows, 64, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    _attend(cache, 1, "bf16", "f32", q)
+    assert int(cache.status) == EINVAL
+
+
+@pytest.mark.gpu
 def test_attend_infinite_and_nan_values_reach_only_rows_that_see_them():
     """Positions no row sees may hold anything; a NaN score is not hidden."""
     cache = Cache([50], [1], "bf16", 16, 1, 64, fill=float("nan"))
@@ -390,7 +407,8 @@ def test_attend_infinite_and_nan_values_reach_only_rows_that_see_them():
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "f16"])
 @pytest.mark.parametrize("heads,kv,dim,new,past", [(2, 1, 64, 5, 40), (8, 2, 128, 9, 300), (4, 4, 96, 7, 5000), (4, 1, 128, 100, 60),
-                                                   (2, 2, 64, 300, 200), (8, 1, 80, 90, 3000)])
+                                                   (2, 2, 64, 300, 200), (8, 1, 80, 90, 3000), (4, 1, 48, 100, 60),
+                                                   (2, 1, 32, 200, 3000), (8, 2, 16, 70, 129)])
 def test_attend_wild_values_of_later_tokens_stay_there(fmt, heads, kv, dim, new, past):
     """A new token whose K and V are infinite or NaN: the rows before it come out as
     without it, it and those after it are not finite."""

@@ -143,10 +143,18 @@ class _Host(vc4b200.GPU):
     (dict(cu=0), "null"), (dict(fed=0), "null"), (dict(logits=0), "null"), (dict(u=0), "null"), (dict(u_sample=0), "null"),
     (dict(next_tokens=0), "null"), (dict(accepted=0), "null"), (dict(logits=66), "aligned"), (dict(probs=66), "aligned"),
     (dict(logits_stride=99), "stride"), (dict(probs_stride=99), "stride"), (dict(work=0), "work buffer"), (dict(work=72), "work buffer"),
-    (dict(work_bytes=1), "work buffer"), ({}, "gpu is null")])
+    (dict(work_bytes=1), "work buffer"),
+    (dict(next_tokens=0x2004), "output overlaps an input"), (dict(accepted=0x1004), "output overlaps an input"),
+    (dict(prob=0x4008), "output overlaps an input"), (dict(work=0x10010), "output overlaps an input"),
+    (dict(next_tokens=0x20100, probs=0x20000), "output overlaps an input"), (dict(status=0x5000), "output overlaps an input"),
+    (dict(accepted=0x6008), "two outputs overlap"), (dict(prob=0x6000), "two outputs overlap"), ({}, "gpu is null"),
+    # neighbours are none of each other's
+    (dict(next_tokens=0x200c, probs=0x20000, prob=0x20000 + 400), "gpu is null")])
 def test_verify_refuses(over, words):
-    a = dict(seqs=1, rows=3, vocab=100, cu=64, fed=64, logits=64, logits_type="f32", temperature=1.0, u=64, u_sample=64,
-             next_tokens=64, accepted=64, prob=0, work=64, work_bytes=1 << 20)
+    a = dict(seqs=1, rows=3, vocab=100, cu=0x1000, fed=0x2000, logits=0x10000, logits_type="f32", temperature=1.0, u=0x4000,
+             u_sample=0x5000, next_tokens=0x6000, accepted=0x7000, prob=0, work=0x30000, work_bytes=1 << 20)
+    if "probs" in over and "next_tokens" in over:
+        a["rows"] = 2 if "prob" in over else 3
     a.update(over)
     with pytest.raises(vc4b200.EngineError) as e:
         _Host().verify_draft(**a)
@@ -311,6 +319,30 @@ def test_verify_nan_infinite_and_unknown_ids(temperature):
     assert st == ERANGE
     _, _, _, st = call([2], [0, -5], lg[3:5], "f32", None, [0.5, 0.5], [0.4], temperature)
     assert st == EINVAL
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu,good", [([0, 3, 2], [0]), ([-1, 3, 6], [1]), ([0, 3, 9], [0]), ([4, 2, 6], [1])])
+def test_verify_flags_bad_offsets(cu, good):
+    """Offsets that run backwards, start below 0 or end past the rows: flagged, the other sequences stand."""
+    g = torch.Generator().manual_seed(2)
+    gpu, vocab, rows = vc4b200.GPU(0), 500, 6
+    lg = torch.randn(rows, vocab, generator=g).cuda()
+    fed = lg.argmax(-1).roll(1).int()
+    ints = torch.full((rows + 4,), -9, dtype=torch.int32, device="cuda")
+    nxt, acc, status = ints[:rows], ints[rows: rows + 2], ints[rows + 2: rows + 3]
+    status.zero_()
+    u, offs = torch.full((rows + 2,), 0.5, device="cuda"), torch.tensor(cu, dtype=torch.int32, device="cuda")
+    need = gpu.verify_bytes(2, rows, vocab)
+    work = torch.zeros(max(16, need), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    gpu.verify_draft(2, rows, vocab, offs.data_ptr(), fed.data_ptr(), lg.data_ptr(), "f32", 0.0, u.data_ptr(),
+                     u[rows:].data_ptr(), nxt.data_ptr(), acc.data_ptr(), 0, work.data_ptr(), need, status=status.data_ptr())
+    gpu.sync()
+    assert int(status) == EINVAL and int(ints[-1]) == -9
+    for s in good:      # every draft is the first maximum of the row before it
+        at = slice(cu[s], cu[s + 1])
+        assert int(acc[s]) == cu[s + 1] - cu[s] - 1 and torch.equal(nxt[at].long(), lg[at].argmax(-1))
 
 
 @pytest.mark.gpu

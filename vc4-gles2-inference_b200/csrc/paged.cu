@@ -3,7 +3,9 @@
 #include "paged.cuh"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
+#include <mutex>
 #include <string>
 
 namespace vc4 {
@@ -95,7 +97,7 @@ __device__ __forceinline__ void store_cache4(uint8_t* row, int i, float4 v) {
 // tokens, by the chain offsets -> length -> page id for a few; the first vectors' loads
 // are issued before that chain.  With one vector at a time the square root, the two
 // divisions and the sums' shuffles, the same for every lane, took as long as the bytes
-// (16384 tokens of 32 + 16 heads of 128 in bf16: 120 us against 78): four
+// (16384 tokens of 32 + 16 heads of 128 in bf16: 120 us against 80): four
 // vectors' sums are halved across the lanes (10 shuffles for 32), so each lane ends with
 // one vector's and takes its root.
 // The float operations are the slot cache's (k_attn): squares summed in double,
@@ -357,6 +359,8 @@ std::string bad_pages(const vc4_pages* p) {
     if (p->pages <= 0 || p->kv_heads <= 0) return "pages and kv_heads must be positive";
     if (p->head_dim <= 0 || p->head_dim > 128 || p->head_dim % 16) return "head_dim must be a multiple of 16, at most 128";
     if (!p->data || !aligned16(p->data)) return "the pool's address must be a multiple of 16";
+    if ((long long)p->pages * 2 > 0x7fffffffLL / ((long long)p->kv_heads * p->page_len))
+        return "a pool holds at most 2^31 - 1 rows (pages x 2 x kv_heads x page_len)";
     return "";
 }
 
@@ -366,6 +370,7 @@ std::string bad_batch(const vc4_paged_batch* b, const vc4_pages* p) {
         return "seqs and table_stride must be positive, tokens, max_new and max_len not negative";
     if (!b->cu || !b->len || !b->table) return "cu, len and table are required";
     if ((long long)b->max_len > (long long)b->table_stride * p->page_len) return "max_len runs past the page table";
+    if ((long long)b->table_stride * p->page_len > (1LL << 30)) return "a page table covers at most 2^30 positions (table_stride x page_len)";
     return "";
 }
 
@@ -423,7 +428,6 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
     } else {
         const int es = p->format == VC4_KV_Q8 ? 1 : 2;
         const long long fit = (long long)sms * split_blocks(es, p->head_dim, pl.wr);
-        pl.splits = 1;
         pl.splits = (int)std::max(1LL, std::min({fit / units, (long long)tiles / 3, (long long)kPagedMaxCluster}));
         if (units < fit && fit / units < kPagedMaxCluster && tiles >= 128 * pl.splits) pl.splits = kPagedMaxCluster;
     }
@@ -531,6 +535,11 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
     if (m.empty()) m = bad_rows("out", out, out_stride, width);
     if (!m.empty()) return refuse(m);
     if (!(scale >= 0.0f) || !(scale < INFINITY)) return refuse("scale must not be negative (0: 1/sqrt(head_dim))");
+    const double grid = p->format == VC4_KV_Q8 ? 1.0 / 16 : p->format == VC4_KV_Q16 ? 1.0 / 2048 : 1.0;
+    const double sc = scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)p->head_dim);
+    const float scale2 = (float)(sc * 1.4426950408889634 * grid);
+    if (!(scale2 >= FLT_MIN) || !(scale2 < INFINITY)) return refuse("scale's product with the pages' grid leaves float's range");
+    if ((long long)b->tokens * heads > 0x7fffffffLL) return refuse("too many rows in one call");
     if (!g) return refuse("gpu is null");
     int sms = 0;
     if (int e = sms_of(gpu_device(g), &sms)) return e;
@@ -546,9 +555,7 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
     a.p = paged_args(p, b);
     a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.q_type = q_type; a.out_type = out_type;
     a.heads = heads; a.group = heads / p->kv_heads; a.row_tiles = pl.row_tiles; a.splits = pl.splits;
-    const double grid = p->format == VC4_KV_Q8 ? 1.0 / 16 : p->format == VC4_KV_Q16 ? 1.0 / 2048 : 1.0;
-    const double sc = scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)p->head_dim);
-    a.scale2 = (float)(sc * 1.4426950408889634 * grid);
+    a.scale2 = scale2;
     a.vscale = (float)grid;
     if (pl.bytes) {
         a.part = (float*)work;

@@ -208,14 +208,15 @@ inline int split_blocks(int es, int hd, int wr) {
 }
 
 // The pool as rows of `row_bytes`; a box is `width` bytes of as many rows as a page has
-// in a tile.  False where no descriptor can be made.
+// in a tile; the host's checks keep the rows below 2^31.  False where no descriptor can
+// be made.
 inline bool paged_map(CUtensorMap* map, const PagedArgs& p, int row_bytes, int width, int tile, CUtensorMapSwizzle swizzle) {
     const auto enc = tmap_encode_fn();
     const int page_len = 1 << p.page_shift, span = page_len < tile ? page_len : tile;
     const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, ((cuuint64_t)p.pages * 2 * p.kv_heads) << p.page_shift};
     const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
     const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)span}, es[2] = {1, 1};
-    return enc && dims[1] <= 0x7fffffffull &&
+    return enc &&
            enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.data, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -246,12 +247,7 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long x, unsigne
     return r;
 }
 
-// Stores 2 or 1 consecutive floats as `type` at element index i of a row.
-__device__ __forceinline__ void store_as(void* row, int type, long long i, float v) {
-    if (type == VC4_F32) reinterpret_cast<float*>(row)[i] = v;
-    else if (type == VC4_BF16) reinterpret_cast<__nv_bfloat16*>(row)[i] = __float2bfloat16_rn(v);
-    else reinterpret_cast<__half*>(row)[i] = __float2half_rn(v);
-}
+// Stores four consecutive floats as `type` from element index i of a row.
 __device__ __forceinline__ void store4_as(void* row, int type, long long i, float4 v) {
     if (type == VC4_F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(row) + i) = v;
     else if (type == VC4_BF16)

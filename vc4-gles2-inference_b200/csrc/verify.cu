@@ -269,9 +269,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
     pdl_wait();
     if (c0 < 0 || n <= 0 || dbase < 0) {   // every block of the cluster leaves here
         if (tid == 0 && writes) a.accepted[s] = 0;
-        if (tid == 0 && n > 0 && a.status) atomicMax(a.status, VC4_EINVAL);   // offsets that run backwards
+        if (tid == 0 && (n || c0 < 0) && a.status) atomicMax(a.status, VC4_EINVAL);   // offsets that run backwards
         return;
     }
+    if (tid == 0 && a.cu[s + 1] > a.rows && a.status) atomicMax(a.status, VC4_EINVAL);
 
     // ---- the walk, W rows at a time, the same in every block ----
     int stop = n - 1, row_first = 0;
@@ -598,6 +599,23 @@ extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const
     const size_t need = (size_t)rows * verify_chunks(rows, vocab) * sizeof(VerifyPart);
     if (work_bytes < need || (need && (!work || (uintptr_t)work % 16)))
         return refuse("the work buffer needs " + std::to_string(need) + " bytes at a multiple of 16");
+    {   // the blocks of a sequence all read the inputs while one of them writes
+        struct Span { const void* at; size_t bytes; };
+        const size_t r = (size_t)rows, n = (size_t)seqs, whole = r > n ? (r - n - 1) * (size_t)probs_stride * 4 + (size_t)vocab * 4 : 0;
+        const Span in[] = {{cu, 4 * (n + 1)}, {fed, 4 * r}, {u, 4 * r}, {u_sample, 4 * n},
+                           {draft_probs, whole}, {logits, r ? ((r - 1) * (size_t)logits_stride + vocab) * es : 0}};
+        const Span out[] = {{next, 4 * r}, {accepted, 4 * n}, {prob, 4 * r}, {status, 4}, {work, need}};
+        auto meet = [](const Span& x, const Span& y) {
+            const uintptr_t a0 = (uintptr_t)x.at, b0 = (uintptr_t)y.at;
+            return a0 && b0 && a0 < b0 + y.bytes && b0 < a0 + x.bytes;
+        };
+        for (const Span& o : out) {
+            for (const Span& i : in)
+                if (meet(o, i)) return refuse("an output overlaps an input");
+            for (const Span& w : out)
+                if (&w != &o && meet(o, w)) return refuse("two outputs overlap");
+        }
+    }
     if (!g) return refuse("gpu is null");
     if (!rows) return VC4_OK;
     int before = -1;
