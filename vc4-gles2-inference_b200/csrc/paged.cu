@@ -44,6 +44,7 @@ struct AppendArgs {
 constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 8;    // most tokens of a block (one warp looks one up)
 constexpr int kAppendVecs = 4;      // head vectors a group of lanes holds at once
+constexpr int kAppendSms = 148;     // SMs the tokens of a block are chosen for
 
 // Four consecutive values of a row, as they lie there and as two float pairs.
 template <int TIN> struct Raw4 { uint2 w; };
@@ -274,13 +275,26 @@ void launch_append_lanes(const AppendArgs& a, int type, unsigned blocks, cudaStr
     else if (type == VC4_BF16) k_paged_append<VC4_BF16, FMT, LPV><<<blocks, kAppendThreads, 0, st>>>(a);
     else k_paged_append<VC4_F16, FMT, LPV><<<blocks, kAppendThreads, 0, st>>>(a);
 }
+int append_lanes(int hd) { return hd > 64 ? 16 : hd > 32 ? 8 : hd > 16 ? 4 : 2; }
 template <int FMT>
 void launch_append(const AppendArgs& a, int type, unsigned blocks, cudaStream_t st) {
-    const int hd = a.p.head_dim;
-    if (hd > 64) launch_append_lanes<FMT, 16>(a, type, blocks, st);
-    else if (hd > 32) launch_append_lanes<FMT, 8>(a, type, blocks, st);
-    else if (hd > 16) launch_append_lanes<FMT, 4>(a, type, blocks, st);
-    else launch_append_lanes<FMT, 2>(a, type, blocks, st);
+    switch (append_lanes(a.p.head_dim)) {
+        case 16: launch_append_lanes<FMT, 16>(a, type, blocks, st); break;
+        case 8: launch_append_lanes<FMT, 8>(a, type, blocks, st); break;
+        case 4: launch_append_lanes<FMT, 4>(a, type, blocks, st); break;
+        default: launch_append_lanes<FMT, 2>(a, type, blocks, st); break;
+    }
+}
+
+// Tokens of a block: what its groups of lanes take in one round, and in three where one
+// round each gives more than six blocks an SM: a block's look-up then comes before more
+// loads (1, 2, 4, 8 tokens: 16384 of 32/8 heads of 128, three rounds at 4, 114, 95, 80,
+// 79 us; 2000 22.7, 22.4, 21.0, 20.5; 600 9.8, 9.4, 11.4, 16.4, one round at 1; 16000 of
+// 4/2 heads of 64, one round at 16, 111, 56, 33, 20).
+int append_tokens(int tokens, int nvec, int hd) {
+    const int groups = kAppendThreads / append_lanes(hd), pieces = (nvec + kAppendVecs - 1) / kAppendVecs;
+    const int rounds = (long long)tokens * pieces / groups > 6 * kAppendSms ? 3 : 1;
+    return std::max(1, std::min(rounds * groups / pieces, kAppendTokens));
 }
 
 // ---------------------------------------------------------------------------
@@ -405,14 +419,17 @@ struct AttnPlan {
 // few-row kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
 // the many-row kernel, 256 a block; of large heads from 33 rows, where every SM has a
 // block (32 x 16 tokens over 4000 bf16 positions, 32/8 heads of 128: 133 us in blocks of
-// 64 rows, 111 in the many-row kernel; 61 x 5 over 2000, 16/2 of 64: 29 and 35).  q16 pages with an f16 or float output stay
-// with the few-row kernel, which holds a level in two operands.
+// 64 rows, 111 in the many-row kernel; 61 x 5 over 2000, 16/2 of 64: 29 and 35).  q16
+// pages with an f16 or float output stay with the few-row kernel, which holds a level in
+// two operands.
 // Splits of the few-row kernel: as many as the GPU holds at once, of three tiles of 64
 // positions or more; a whole cluster of eight for long sequences that do not fill the GPU
 // a whole number of times, whose ragged lengths then even out (12 x 40k positions: 1, 2,
-// 3, 4, 8 splits 457, 274, 283, 278, 244 us).  Of the many-row kernel: what
-// one block on each SM allows, of eight tiles of 128 or more; they leave partial results in the work buffer, for a second
-// kernel.
+// 3, 4, 8 splits 457, 274, 283, 278, 244 us).  Of the many-row kernel: what one block on
+// each SM allows, down to one tile of 128 (8, 4, 2, 1 tiles or more: 128 tokens over 2000
+// bf16 positions, 32/8 heads of 128, 32.9, 26.7, 24.7, 25.0 us; 300 over 1500 q16, 8/4 of
+// 96, 51.5, 29.8, 24.1, 24.7; 128 over 700 24.9, 24.9, 24.7, 21.0); they leave partial
+// results in the work buffer, for a second kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
     const long long rows = (long long)b->max_new * (heads / p->kv_heads);
@@ -424,7 +441,7 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
     const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
     const int tiles = (b->max_len + tile - 1) / tile;
     if (pl.chunk) {
-        pl.splits = (int)std::max(1LL, std::min({sms / units, (long long)tiles / 8, (long long)kPagedMaxSplits}));
+        pl.splits = (int)std::max(1LL, std::min({sms / units, (long long)tiles, (long long)kPagedMaxSplits}));
     } else {
         const int es = p->format == VC4_KV_Q8 ? 1 : 2;
         const long long fit = (long long)sms * split_blocks(es, p->head_dim, pl.wr);
@@ -486,9 +503,7 @@ extern "C" int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_
     a.qkv = qkv; a.q = q; a.qkv_stride = qkv_stride; a.q_stride = q_stride;
     a.q_norm = q_norm; a.k_norm = k_norm; a.cos = cos; a.sin = sin; a.eps = eps;
     a.heads = heads; a.rope_len = rope_len; a.half = rope_half ? 1 : 0; a.q_type = q_type;
-    // one token per block while the blocks fit the GPU at once, then more, so
-    // that a block's look-up is shared by several rounds of vectors
-    a.per_block = b->tokens <= 1024 ? 1 : b->tokens <= 4096 ? 2 : 4;
+    a.per_block = append_tokens(b->tokens, heads + 2 * p->kv_heads, p->head_dim);
     const unsigned blocks = (unsigned)(((long long)b->tokens + a.per_block - 1) / a.per_block);
     switch (pfmt(p->format)) {
         case P_Q8: launch_append<P_Q8>(a, qkv_type, blocks, st); break;
