@@ -98,7 +98,7 @@ __device__ __forceinline__ void store_cache4(uint8_t* row, int i, float4 v) {
 // tokens, by the chain offsets -> length -> page id for a few; the first vectors' loads
 // are issued before that chain.  With one vector at a time the square root, the two
 // divisions and the sums' shuffles, the same for every lane, took as long as the bytes
-// (16384 tokens of 32 + 16 heads of 128 in bf16: 120 us against 80): four
+// (12332 tokens of 32 + 16 heads of 128 in bf16: 120 us against 80, 3.8 TB/s): four
 // vectors' sums are halved across the lanes (10 shuffles for 32), so each lane ends with
 // one vector's and takes its root.
 // The float operations are the slot cache's (k_attn): squares summed in double,
@@ -288,8 +288,8 @@ void launch_append(const AppendArgs& a, int type, unsigned blocks, cudaStream_t 
 
 // Tokens of a block: what its groups of lanes take in one round, and in three where one
 // round each gives more than six blocks an SM: a block's look-up then comes before more
-// loads (1, 2, 4, 8 tokens: 16384 of 32/8 heads of 128, three rounds at 4, 114, 95, 80,
-// 79 us; 2000 22.7, 22.4, 21.0, 20.5; 600 9.8, 9.4, 11.4, 16.4, one round at 1; 16000 of
+// loads (1, 2, 4, 8 tokens: 12332 of 32/8 heads of 128, three rounds at 4, 114, 95, 80,
+// 79 us; 2000 22.7, 22.4, 21.0, 20.5; 600 9.8, 9.4, 11.4, 16.4, one round at 1; 14204 of
 // 4/2 heads of 64, one round at 16, 111, 56, 33, 20).
 int append_tokens(int tokens, int nvec, int hd) {
     const int groups = kAppendThreads / append_lanes(hd), pieces = (nvec + kAppendVecs - 1) / kAppendVecs;
@@ -302,7 +302,8 @@ int append_tokens(int tokens, int nvec, int hd) {
 // ---------------------------------------------------------------------------
 
 // One warp per (token, head); lane i holds the weights of splits i and i + 32, then four
-// values of the row.
+// values of the row.  Bound by the partial sums' bytes, which the many-row kernel just
+// left in L2 (256 tokens x 16 heads of 128 in 9 parts: 7.8 us).
 __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
     pdl_wait();
     const int lane = threadIdx.x & 31;
