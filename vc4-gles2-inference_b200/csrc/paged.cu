@@ -424,13 +424,17 @@ struct AttnPlan {
 // pages with an f16 or float output stay with the few-row kernel, which holds a level in
 // two operands.
 // Splits of the few-row kernel: as many as the GPU holds at once, of three tiles of 64
-// positions or more; a whole cluster of eight for long sequences that do not fill the GPU
-// a whole number of times, whose ragged lengths then even out (12 x 40k positions: 1, 2,
-// 3, 4, 8 splits 457, 274, 283, 278, 244 us).  Of the many-row kernel: what one block on
-// each SM allows, down to one tile of 128 (8, 4, 2, 1 tiles or more: 128 tokens over 2000
-// bf16 positions, 32/8 heads of 128, 32.9, 26.7, 24.7, 25.0 us; 300 over 1500 q16, 8/4 of
-// 96, 51.5, 29.8, 24.1, 24.7; 128 over 700 24.9, 24.9, 24.7, 21.0); they leave partial
-// results in the work buffer, for a second kernel.
+// positions or more (16 rows, whose four warps share a tile; 32 rows two, 64 rows, where
+// each warp takes every tile, one): in a replayed graph, with 1, 2, 3, 6 tiles a split,
+// one token over 777 q16 positions 11.6, 11.0, 10.3, 11.3 us, 16 x 8 over 300, 16/4 heads
+// of 64, 8.9, 8.3, 8.7, 8.7, 5 over 400, 16/2 of 64, 7.9, 9.9, 10.3, 13.1; a whole
+// cluster of eight for long sequences that do not fill the GPU a whole number of times,
+// whose ragged lengths then even out (12 x 40k positions: 1, 2, 3, 4, 8 splits 457, 274,
+// 283, 278, 244 us).  Of the many-row kernel: what one block on each SM allows, down to
+// one tile of 128 (8, 4, 2, 1 tiles or more: 128 tokens over 2000 bf16 positions, 32/8
+// heads of 128, 32.9, 26.7, 24.7, 25.0 us; 300 over 1500 q16, 8/4 of 96, 51.5, 29.8,
+// 24.1, 24.7; 128 over 700 24.9, 24.9, 24.7, 21.0); they leave partial results in the
+// work buffer, for a second kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
     const long long rows = (long long)b->max_new * (heads / p->kv_heads);
@@ -446,7 +450,8 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
     } else {
         const int es = p->format == VC4_KV_Q8 ? 1 : 2;
         const long long fit = (long long)sms * split_blocks(es, p->head_dim, pl.wr);
-        pl.splits = (int)std::max(1LL, std::min({fit / units, (long long)tiles / 3, (long long)kPagedMaxCluster}));
+        const int least = pl.wr == 1 ? 3 : pl.wr == 2 ? 2 : 1;
+        pl.splits = (int)std::max(1LL, std::min({fit / units, (long long)tiles / least, (long long)kPagedMaxCluster}));
         if (units < fit && fit / units < kPagedMaxCluster && tiles >= 128 * pl.splits) pl.splits = kPagedMaxCluster;
     }
     if (pl.chunk && pl.splits > 1) pl.bytes = (size_t)pl.splits * b->tokens * heads * ((size_t)p->head_dim * 4 + 8);
