@@ -492,3 +492,29 @@ def test_pages_hold_the_slot_caches_rows(tiny_paths, key):
     want = reference([4], toks[-4:], lg, None, u, [0.5], 1.0)
     got = call([4], np.array(toks[-4:]), ints, "q16", None, u, np.array([0.5], np.float32), 1.0)
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+# ---- ends of the ranges -----------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,top", [("f32", -3.4e38), ("f32", 1e20), ("f32", -65504.0), ("f32", 3e38), ("bf16", None), ("f16", None)])
+@pytest.mark.parametrize("temperature", [0.7, 1.0, 1e-5, 50.0])
+def test_verify_rows_of_huge_finite_logits(kind, top, temperature):
+    """A row's largest logit is weighed 1 wherever it lies: all ids masked with the
+    type's lowest value are equally likely, and one that stands out takes all."""
+    vocab, low = 1500, torch.finfo(TORCH[kind]).min
+    lg = torch.full((4, vocab), low if top is None else top, dtype=TORCH[kind])     # rows 0, 1: equal
+    lg[2:, :] = low
+    lg[2:, 700] = low / 2 if top is None or top == -3.4e38 else top      # rows 2, 3: one stands out, by far
+    counts, fed, u, us = [1, 1, 2], [0, 0, 0, 700], np.full(4, 0.999, np.float32), np.array([0.2501, 0.9, 0.5], np.float32)
+    want = reference(counts, fed, lg.double().numpy(), None, u, us, temperature)
+    assert want[3] and want[0].tolist() == [375, 1349, 700, 700]
+    got = call(counts, fed, lg, kind, None, u, us, temperature)
+    assert got[3] == 0 and np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    assert np.all(np.abs(got[2] - want[2]) <= 2.0 ** -19 * want[2])
+    # what is left of p behind draft probabilities: the row's own p below them at one id
+    d = torch.full((1, vocab), 1 / vocab)
+    d[0, :vocab // 2] = 0
+    want = reference([2], [0, 1000], lg[:2].double().numpy(), d.numpy(), [1.5, 0], us[:1], temperature)
+    got = call([2], [0, 1000], lg[:2], kind, d, [1.5, 0], us[:1], temperature)
+    assert want[3] and got[3] == 0 and np.array_equal(got[0], want[0]) and want[0][0] < vocab // 2

@@ -369,13 +369,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
     const bool refused = stop < n - 1;
     const float* drow = refused && a.probs ? a.probs + (long long)(dbase + stop) * a.probs_stride : nullptr;
     const int cut = refused && !a.probs ? a.fed[row + 1] : -1;
-    // exp((l - max)/T); the product's rounding, one for all ids, shifts every weight by
-    // less than 1e-14 of it.  Infinite maxima take all, in equal parts.
+    // exp((l - max)/T), the difference taken first: the maximum's weight is 1 however large
+    // it is.  Infinite maxima take all, in equal parts.
     const bool endless = row_max == INFINITY;
-    const double scale = a.scale256, shift = endless ? 0.0 : -(double)row_max * scale;
+    const double scale = a.scale256, most = endless ? 0.0 : (double)row_max;
     auto weight = [&](float l) -> double {
         if (endless) l = l == row_max ? 0.0f : -INFINITY;
-        return exp2_256(fma((double)l, scale, shift), s_tab);
+        return exp2_256(((double)l - most) * scale, s_tab);
     };
     const float inv0 = (float)(1.0 / row_sum);
     const bool dvec = (((uintptr_t)drow - 4 * r.head) & 15) == 0;   // words of logits meet 16-byte pieces of d
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
                 }
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const double e = exp2_256(fma((double)l[j], scale, shift), s_tab);
+                    const double e = exp2_256(((double)l[j] - most) * scale, s_tab);
                     S += e;
                     if (rule == 1 && wk * VEC - r.head + j != cut) E += e;
                     if (rule == 2 && (float)e * inv0 > d[k][j]) {
