@@ -406,7 +406,8 @@ VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_
    maximum; else 1e-5 or more).  The draft after row i of sequence s (the next fed
    id, x) is accepted while u[row] * d(x) < p(x), d being the draft's row of
    draft_probs (one row for each draft of the batch in order, probs_stride apart; 0:
-   vocab), or one at x and zero elsewhere when draft_probs is NULL.  The first
+   vocab; sequences behind offsets that start below 0 or run backwards are skipped, for
+   their rows of it are unknown), or one at x and zero elsewhere when draft_probs is NULL.  The first
    refused row is sampled from max(p - d, 0) normalised (from p where that is zero
    everywhere), and the last row, when all are accepted, from p:
    the first id whose cumulative sum exceeds u_sample[s] times the total, sums in

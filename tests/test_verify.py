@@ -518,3 +518,62 @@ def test_verify_rows_of_huge_finite_logits(kind, top, temperature):
     want = reference([2], [0, 1000], lg[:2].double().numpy(), d.numpy(), [1.5, 0], us[:1], temperature)
     got = call([2], [0, 1000], lg[:2], kind, d, [1.5, 0], us[:1], temperature)
     assert want[3] and got[3] == 0 and np.array_equal(got[0], want[0]) and want[0][0] < vocab // 2
+
+
+def _offsets(cu, rows, vocab, drafts, seed=2):
+    """One greedy call over `rows` rows with offsets of any kind and `drafts` rows of draft
+    probabilities: all 1 at the draft, so a draft is accepted where u < p.  Returns (logits,
+    next, accepted, status)."""
+    g = torch.Generator().manual_seed(seed)
+    gpu, seqs = vc4b200.GPU(0), len(cu) - 1
+    lg = torch.randn(rows, vocab, generator=g).cuda()
+    fed = lg.argmax(-1).roll(1).int()
+    nxt, acc = (torch.full((n,), -9, dtype=torch.int32, device="cuda") for n in (rows, seqs))
+    status, offs = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.tensor(cu, dtype=torch.int32, device="cuda")
+    u, us = torch.full((rows,), 0.5, device="cuda"), torch.full((seqs,), 0.5, device="cuda")
+    need = gpu.verify_bytes(seqs, rows, vocab)
+    work = torch.zeros(max(16, need), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    gpu.verify_draft(seqs, rows, vocab, offs.data_ptr(), fed.data_ptr(), lg.data_ptr(), "f32", 0.0, u.data_ptr(), us.data_ptr(),
+                     nxt.data_ptr(), acc.data_ptr(), 0, work.data_ptr(), need, probs=drafts.data_ptr(), status=status.data_ptr())
+    gpu.sync()
+    return lg, nxt, acc, int(status)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [0, 1, 5])
+def test_verify_draft_rows_count_from_the_first_offset(first):
+    """A batch whose first sequence starts at row `first`: its draft probabilities are rows
+    0, 1, .. of the array, which ends with the last draft."""
+    vocab, counts = 300, [3, 0, 1, 4]
+    cu = np.concatenate([[0], np.cumsum(counts)]) + first
+    drafts = torch.zeros(5, vocab, device="cuda")
+    drafts[[0, 2, 3]] = 1.0            # rows 1 and 4: d is 3, so u * d is above any p
+    drafts[[1, 4]] = 3.0
+    lg, nxt, acc, status = _offsets(cu.tolist(), first + 8, vocab, drafts)
+    assert status == 0 and acc.tolist() == [1, 0, 0, 2]
+    want = lg.argmax(-1).int()
+    assert nxt[:first].tolist() == [-9] * first
+    # (a refused row's p is one at its maximum, where d is above it: the rest falls back to p)
+    for at, n, a in ((first, 3, 1), (first + 3, 1, 0), (first + 4, 4, 2)):
+        assert torch.equal(nxt[at: at + a + 1], want[at: at + a + 1]) and bool((nxt[at + a + 1: at + n] == -1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu,good,drafts", [([0, 3, 2], [0], 2), ([-1, 3, 6], [], 5), ([0, 3, 9], [0, 1], 4), ([4, 2, 6], [], 3),
+                                            ([0, 9, 3, 6], [0], 5), ([0, 2, 1, 4, 6], [0], 4)])
+def test_verify_skips_draft_rows_behind_bad_offsets(cu, good, drafts):
+    """With draft probabilities: sequences behind offsets that start below 0 or run backwards
+    are flagged and skipped, those before them stand."""
+    rows, vocab = 6, 300
+    lg, nxt, acc, status = _offsets(cu, rows, vocab, torch.ones(drafts, vocab, device="cuda"))
+    assert status == EINVAL
+    touched = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for s in range(len(cu) - 1):
+        at = slice(max(0, cu[s]), max(0, min(cu[s + 1], rows)))
+        if s in good:       # every draft is the first maximum of the row before it
+            assert int(acc[s]) == at.stop - at.start - 1 and torch.equal(nxt[at].long(), lg[at].argmax(-1))
+            touched[at] = True
+        else:
+            assert int(acc[s]) == 0
+    assert bool((nxt[~touched] == -9).all())

@@ -260,16 +260,25 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
     const int s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c0 = a.cu[s], c1 = min(a.cu[s + 1], a.rows), n = c1 - c0, V = a.vocab;
     s_tab[tid] = exp2((double)tid / 256);
-    // this sequence's first row of draft_probs: a row for each before it, but for
-    // the last row of every sequence that has any
-    int dbase = c0;
-    if (a.probs)
-        for (int j = 0; j < s; j += kVerifyThreads)
-            dbase -= __syncthreads_count(j + tid < s && a.cu[j + tid + 1] > a.cu[j + tid]);
+    // this sequence's first row of draft_probs: a row for each of the batch before it, but
+    // for the last row of every sequence that has any.  Behind offsets that start below 0 or
+    // run backwards nobody knows where it is.
+    int dbase = 0;
+    bool lost = false;
+    if (a.probs) {
+        const int first = a.cu[0];
+        dbase = c0 - first;
+        lost = first < 0;
+        for (int j = 0; j < s; j += kVerifyThreads) {
+            const int i = min(j + tid, s - 1), lo = a.cu[i], hi = a.cu[i + 1];
+            lost |= hi < lo;
+            dbase -= __syncthreads_count(j + tid < s && hi > lo);
+        }
+    }
     const bool writes = rank == 0;
-    __syncthreads();
+    lost = __syncthreads_or(lost);
     pdl_wait();
-    if (c0 < 0 || n <= 0 || dbase < 0) {   // every block of the cluster leaves here
+    if (c0 < 0 || n <= 0 || lost) {        // every block of the cluster leaves here
         if (tid == 0 && writes) a.accepted[s] = 0;
         if (tid == 0 && (n || c0 < 0) && a.status) atomicMax(a.status, VC4_EINVAL);   // offsets that run backwards
         return;
