@@ -547,3 +547,77 @@ def test_no_tokens_and_work_buffer():
     handle.append(empty, q.data_ptr(), "bf16", 4, out.data_ptr(), "f32")
     torch.cuda.synchronize()
     assert bool((out == 0).all())
+
+
+# ---- offsets of any kind ------------------------------------------------------------------
+
+OFFSETS = [  # offsets of two or three sequences over 6 rows, those that stand
+    ([0, 3, 9], [0]), ([0, 3, 2], [0]), ([-1, 3, 6], [1]), ([-2, -1, 6], []), ([4, 2, 6], [1]), ([0, 3, 1, 6], []),
+    ([0, 2, 7, 7], [0]), ([0, 6, 4], [0])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu,good", OFFSETS)
+@pytest.mark.parametrize("fmt", ["q8", "bf16"])
+def test_append_flags_bad_offsets(fmt, cu, good):
+    """Offsets that start below 0, run backwards or end past the rows: flagged; a sequence
+    with such an offset writes nothing, the others what they write alone.  (Rows of two
+    sequences that overlap belong to one of them.)"""
+    seqs, heads, kv, dim = len(cu) - 1, 4, 2, 64
+    cache = Cache([40] * seqs, [3] * seqs, fmt, 16, kv, dim, rows=6)
+    cache.new = [6] * seqs                       # max_new of the batch: no bound of its own here
+    t, kw = _append_case(cache, heads, "f32", "bf16", True, True)
+    gpu = vc4b200.GPU(0)
+    cache.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+    handle, batch = cache.handles(vc4b200, gpu)
+    before = cache.pool.clone()
+    torch.cuda.synchronize()
+    handle.append(batch, t["qkv"].data_ptr(), "f32", heads, t["q"].data_ptr(), "bf16", **kw)
+    gpu.sync()
+    assert int(cache.status) == EINVAL
+    pages = lambda s: torch.from_numpy(cache.host_table[s, :3].astype(np.int64)).cuda()  # noqa: E731
+    for s in range(seqs):
+        now, was = cache.pool[pages(s)], before[pages(s)]
+        if 0 <= cu[s] <= cu[s + 1] <= 6 and s in good:
+            n = cu[s + 1] - cu[s]
+            alone = Cache([40], [n], fmt, 16, kv, dim, rows=6)
+            alone.pool, alone.pages = before.clone(), cache.pages
+            alone.table.copy_(cache.table[s: s + 1])
+            alone.cu.copy_(torch.tensor([cu[s], cu[s + 1]], dtype=torch.int32))
+            h, b = alone.handles(vc4b200, gpu)
+            q = torch.full_like(t["q"], 7.0)
+            torch.cuda.synchronize()
+            h.append(b, t["qkv"].data_ptr(), "f32", heads, q.data_ptr(), "bf16", **kw)
+            gpu.sync()
+            assert int(alone.status) == 0 and torch.equal(now, alone.pool[pages(s)])
+            assert torch.equal(t["q"][cu[s]: cu[s + 1]], q[cu[s]: cu[s + 1]])
+        elif not (0 <= cu[s] <= cu[s + 1] <= 6):
+            assert torch.equal(now, was)
+    inside = torch.zeros(6, dtype=torch.bool, device="cuda")
+    for s in range(seqs):
+        if 0 <= cu[s] <= cu[s + 1] <= 6:
+            inside[cu[s]: cu[s + 1]] = True
+    assert bool((t["q"][~inside] == 7).all())
+
+
+@pytest.mark.gpu
+def test_append_flags_a_bad_offset_among_many_sequences():
+    """The offset that runs backwards lies past every row: no token's look-up meets it."""
+    seqs = 3000
+    cache = Cache([20] * 2, [1] * 2, "q8", 16, 1, 16, rows=2)
+    cu = torch.full((seqs + 1,), 2, dtype=torch.int32, device="cuda")
+    cu[0], cu[1] = 0, 1
+    length = torch.full((seqs,), 20, dtype=torch.int32, device="cuda")
+    table = cache.table[:1].repeat(seqs, 1).contiguous()
+    t, kw = _append_case(cache, 1, "f32", "f32", False, True)
+    gpu = vc4b200.GPU(0)
+    handle, _ = cache.handles(vc4b200, gpu)
+    for bad in (False, True):
+        if bad:
+            cu[2900] = 1
+        batch = vc4b200.PagedBatch(cu.data_ptr(), length.data_ptr(), table.data_ptr(), seqs, 2, 1, 20, cache.width,
+                                   status=cache.status.data_ptr())
+        torch.cuda.synchronize()
+        handle.append(batch, t["qkv"].data_ptr(), "f32", 1, t["q"].data_ptr(), "f32", **kw)
+        gpu.sync()
+        assert int(cache.status) == (EINVAL if bad else 0)

@@ -133,6 +133,11 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
     const int first = warp * NG + lane / LPV;
     fetch(first);
 
+    // offsets that start below 0, run backwards or end past the rows, wherever a token's look-up
+    // does not meet them: a sequence a thread
+    if (p.status)
+        for (long long i = (long long)blockIdx.x * kAppendThreads + threadIdx.x; i < p.seqs; i += (long long)gridDim.x * kAppendThreads)
+            if (p.cu[i] < 0 || p.cu[i + 1] < p.cu[i] || p.cu[i + 1] > p.tokens) paged_flag(p.status, VC4_EINVAL);
     if (warp < ntok) {
         const int tok = tok0 + warp, s = paged_find(p.cu, p.seqs, tok);
         const int c0 = p.cu[s], c1 = p.cu[s + 1];
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
             const int page_len = 1 << p.page_shift;
             pos = p.len[s] - (c1 - tok);
             bool bad = pos < 0 || pos >= (long long)p.table_stride * page_len || (a.cos && pos >= a.rope_len) ||
-                       c1 - c0 > p.max_new;
+                       c1 - c0 > p.max_new || c0 < 0 || c1 > p.tokens;
             if (!bad) {
                 const int page = p.table[(size_t)s * p.table_stride + (pos >> p.page_shift)];
                 bad = page < 0 || page >= p.pages;
