@@ -621,3 +621,32 @@ def test_append_flags_a_bad_offset_among_many_sequences():
         handle.append(batch, t["qkv"].data_ptr(), "f32", 1, t["q"].data_ptr(), "f32", **kw)
         gpu.sync()
         assert int(cache.status) == (EINVAL if bad else 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cu,good", [((0, 100, 201), [0, 1]), ((-1, 100, 200), [1]), ((0, 100, 1), [0]), ((100, 100, 200), [0, 1]),
+                                     ((-5, -1, 200), [])])
+@pytest.mark.parametrize("heads,length", [(1, 300), (4, 3000), (8, 130)])
+def test_attend_leaves_rows_of_bad_offsets(heads, length, cu, good):
+    """Many rows, their positions split or not: a sequence that starts below 0 or ends before
+    it starts is skipped, its rows and those behind the batch stay; the others are the
+    definition's, one that runs past the rows with the rows there are."""
+    new, dim = 100, 64
+    cache = Cache([length, length - 90], [new, new], "bf16", 16, 1, dim, rows=2 * new)
+    # (a length below the new tokens is flagged too: 40 positions for 100 tokens)
+    bad = not 0 <= cu[0] <= cu[1] <= cu[2] <= 2 * new or length - 90 < cu[2] - cu[1]
+    cache.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+    q = torch.randn(2 * new, heads * dim, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    out, _ = _attend(cache, heads, "bf16", "f32", q)
+    assert int(cache.status) == (EINVAL if bad else 0)
+    left = torch.ones(2 * new, dtype=torch.bool, device="cuda")
+    cache.host_cu = np.maximum(0, np.minimum(cu, 2 * new))
+    cache.new = [max(0, int(n)) if s in good else 0 for s, n in enumerate(cache.host_cu[1:] - cache.host_cu[:-1])]
+    cache.tokens = 2 * new
+    want, mass, top = attention(cache, q, heads)
+    bound = attention_bound("bf16", "f32", want, mass, top, dim)
+    for s in good:
+        rows = slice(int(cache.host_cu[s]), int(cache.host_cu[s]) + cache.new[s])
+        assert bool(((out[rows].double().view_as(want[rows]) - want[rows]).abs() <= bound[rows]).all())
+        left[rows] = False
+    assert bool((out[left] == 7).all())

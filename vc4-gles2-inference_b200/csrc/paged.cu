@@ -321,9 +321,10 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         e[k] = lane + 32 * k < a.splits ? a.ml[at + (lane + 32 * k) * step] : make_float2(-INFINITY, 0.0f);
-    // rows behind the last sequence, and those beyond max_new, were not computed: leave them
-    const int s = paged_find(p.cu, p.seqs, tok);
-    if (tok < p.cu[s] || tok >= p.cu[s + 1] || tok - p.cu[s] >= p.max_new) return;
+    // rows behind the last sequence, those of a sequence that starts below 0 and those beyond
+    // max_new were not computed: leave them
+    const int s = paged_find(p.cu, p.seqs, tok), c0 = p.cu[s];
+    if (c0 < 0 || tok < c0 || tok >= p.cu[s + 1] || tok - c0 >= p.max_new) return;
     float m = fmaxf(e[0].x, e[1].x);
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float w[2], l = 0.0f;
