@@ -412,7 +412,7 @@ VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_
    everywhere), and the last row, when all are accepted, from p:
    the first id whose cumulative sum exceeds u_sample[s] times the total, sums in
    double.  next: per row the accepted draft, then the sampled id, then -1;
-   accepted (seqs): drafts accepted; prob (rows, or NULL): the target's probability
+   accepted (seqs): drafts accepted, 0 for a sequence without rows; prob (rows, or NULL): the target's probability
    of each id in next, 0 where that is -1.  logits_type: VC4_F32, VC4_BF16, VC4_F16
    or VC4_Q16I.  `rows` bounds cu[seqs].  NaN logits count as -inf.  An output that
    overlaps an input or another output is refused. */

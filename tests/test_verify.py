@@ -577,3 +577,27 @@ def test_verify_skips_draft_rows_behind_bad_offsets(cu, good, drafts):
         else:
             assert int(acc[s]) == 0
     assert bool((nxt[~touched] == -9).all())
+
+
+@pytest.mark.gpu
+def test_verify_without_any_row_accepts_nothing():
+    """No sequence has a row: the counts are 0 all the same, captured too."""
+    gpu = vc4b200.GPU(0)
+    ints = lambda n, v: torch.full((n,), v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cu, fed, nxt, acc, lg = ints(4, 0), ints(4, 0), ints(4, -9), ints(4, -9), torch.zeros(4, 100, device="cuda")
+    u = torch.zeros(4, device="cuda")
+    assert gpu.verify_bytes(3, 0, 100) == 0
+
+    def step():
+        gpu.verify_draft(3, 0, 100, cu.data_ptr(), fed.data_ptr(), lg.data_ptr(), "f32", 1.0, u.data_ptr(), u.data_ptr(),
+                         nxt.data_ptr(), acc.data_ptr(), 0, 0, 0, stream=torch.cuda.current_stream().cuda_stream)
+    step()
+    torch.cuda.synchronize()
+    assert acc.tolist() == [0, 0, 0, -9] and nxt.tolist() == [-9] * 4
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    acc.fill_(5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert acc.tolist() == [0, 0, 0, 5]

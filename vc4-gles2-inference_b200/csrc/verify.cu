@@ -628,13 +628,17 @@ extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const
         }
     }
     if (!g) return refuse("gpu is null");
-    if (!rows) return VC4_OK;
     int before = -1;
     cudaError_t e = cudaGetDevice(&before);
     if (e == cudaSuccess && before != gpu_device(g)) e = cudaSetDevice(gpu_device(g));
     else before = -1;
     if (e != cudaSuccess) return vfail(VC4_ECUDA, cudaGetErrorString(e));
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : gpu_stream(g);
+    if (!rows) {     // no sequence has a row: none accepts a draft
+        e = cudaMemsetAsync(accepted, 0, (size_t)seqs * sizeof(int), st);
+        if (before >= 0) cudaSetDevice(before);
+        return e == cudaSuccess ? VC4_OK : vfail(VC4_ECUDA, std::string("verify_draft: ") + cudaGetErrorString(e));
+    }
     VerifyArgs a{};
     a.seqs = seqs; a.rows = rows; a.vocab = vocab;
     a.cu = cu; a.fed = fed; a.logits = logits; a.stride = logits_stride; a.probs_stride = probs_stride;
