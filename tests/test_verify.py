@@ -601,3 +601,14 @@ def test_verify_without_any_row_accepts_nothing():
     graph.replay()
     torch.cuda.synchronize()
     assert acc.tolist() == [0, 0, 0, 5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("x", [300, 2 ** 31 - 1, -1, -2 ** 31])
+def test_verify_never_accepts_an_unknown_id(x, temperature):
+    """An id outside the vocabulary is refused whatever u says, and not handed on."""
+    lg = torch.randn(3, 300, generator=torch.Generator().manual_seed(4))
+    nxt, acc, prob, st = call([3], [0, x, 1], lg, "f32", None, [-1.0, 0.5, 0], [0.4], temperature)
+    want = reference([3], [0, x, 1], lg.numpy(), None, [1.0, 0.5, 0], [np.float32(0.4)], temperature)
+    assert st == EINVAL and acc[0] == 0 and np.array_equal(nxt, want[0]) and 0 <= nxt[0] < 300

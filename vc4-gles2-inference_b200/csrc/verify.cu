@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
                 s_max[warp] = top;
                 s_rowsum[warp] = sum;
                 s_first[warp] = first;
-                s_ok[warp] = judge && (double)u * (double)d < q;
+                s_ok[warp] = judge && in && (double)u * (double)d < q;
                 s_p[warp] = (float)q;
                 if (writes && a.status) {
                     if (!in) atomicMax(a.status, VC4_EINVAL);
