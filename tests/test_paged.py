@@ -650,3 +650,12 @@ def test_attend_leaves_rows_of_bad_offsets(heads, length, cu, good):
         assert bool(((out[rows].double().view_as(want[rows]) - want[rows]).abs() <= bound[rows]).all())
         left[rows] = False
     assert bool((out[left] == 7).all())
+
+
+@pytest.mark.parametrize("name", ["cu", "length", "table", "status"])
+@pytest.mark.parametrize("off", [1, 2])
+def test_batches_off_their_elements_are_refused(name, off):
+    batch = _host_batch(**{name: 64 + off})
+    _refused(lambda: _host_pages().append(batch, 64, "f32", 4, 64, "bf16"), "aligned to their elements")
+    _refused(lambda: _host_pages().attend(batch, 64, "bf16", 4, 64, "bf16"), "aligned to their elements")
+    _refused(lambda: _host_pages().attend_bytes(batch, 4), "aligned to their elements")

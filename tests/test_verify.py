@@ -612,3 +612,14 @@ def test_verify_never_accepts_an_unknown_id(x, temperature):
     nxt, acc, prob, st = call([3], [0, x, 1], lg, "f32", None, [-1.0, 0.5, 0], [0.4], temperature)
     want = reference([3], [0, x, 1], lg.numpy(), None, [1.0, 0.5, 0], [np.float32(0.4)], temperature)
     assert st == EINVAL and acc[0] == 0 and np.array_equal(nxt, want[0]) and 0 <= nxt[0] < 300
+
+
+@pytest.mark.parametrize("name", ["cu", "fed", "probs", "u", "u_sample", "next_tokens", "accepted", "prob", "status"])
+@pytest.mark.parametrize("off", [1, 2])
+def test_verify_refuses_arrays_off_their_elements(name, off):
+    a = dict(seqs=1, rows=3, vocab=100, cu=0x1000, fed=0x2000, logits=0x10000, logits_type="f32", temperature=1.0, u=0x4000,
+             u_sample=0x5000, next_tokens=0x6000, accepted=0x7000, prob=0x8000, work=0x30000, work_bytes=1 << 20, probs=0x20000,
+             status=0x9000)
+    a[name] += off
+    with pytest.raises(vc4b200.EngineError, match="error %d.*aligned" % EINVAL):
+        _Host().verify_draft(**a)

@@ -390,6 +390,8 @@ std::string bad_batch(const vc4_paged_batch* b, const vc4_pages* p) {
     if (b->seqs <= 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_stride <= 0)
         return "seqs and table_stride must be positive, tokens, max_new and max_len not negative";
     if (!b->cu || !b->len || !b->table) return "cu, len and table are required";
+    if (((uintptr_t)b->cu | (uintptr_t)b->len | (uintptr_t)b->table | (uintptr_t)b->status) % 4)
+        return "cu, len, table and status are aligned to their elements";
     if ((long long)b->max_len > (long long)b->table_stride * p->page_len) return "max_len runs past the page table";
     if ((long long)b->table_stride * p->page_len > (1LL << 30)) return "a page table covers at most 2^30 positions (table_stride x page_len)";
     return "";

@@ -606,7 +606,10 @@ extern "C" int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const
         return refuse("temperature must be 0 or at least 1e-5");
     if (!cu || !fed || !logits || !u || !u_sample || !next || !accepted) return refuse("a required array is null");
     const int es = logits_type == VC4_BF16 || logits_type == VC4_F16 ? 2 : 4;
-    if ((uintptr_t)logits % es || (uintptr_t)draft_probs % 4) return refuse("an array is not aligned to its elements");
+    const void* words[] = {cu, fed, draft_probs, u, u_sample, next, accepted, prob, status};
+    bool aligned = (uintptr_t)logits % es == 0;
+    for (const void* w : words) aligned = aligned && (uintptr_t)w % 4 == 0;
+    if (!aligned) return refuse("an array is not aligned to its elements");
     const size_t need = (size_t)rows * verify_chunks(rows, vocab) * sizeof(VerifyPart);
     if (work_bytes < need || (need && (!work || (uintptr_t)work % 16)))
         return refuse("the work buffer needs " + std::to_string(need) + " bytes at a multiple of 16");
