@@ -373,8 +373,9 @@ typedef struct {
    the sequence's page, the rotated q to q ([heads][head_dim], q_stride apart).
    The operations and their order are the slot cache's, so the page bytes of the
    q8 / q16 formats are those vc4_kv_read_rows gives.  qkv_type and q_type:
-   VC4_F32, VC4_BF16 or VC4_F16.  Two sequences must not append into one page, and
-   q must not overlap qkv.
+   VC4_F32, VC4_BF16 or VC4_F16.  Two sequences must not append into one page.  A q
+   that overlaps qkv, and a pool that overlaps either, is refused (rows side by side in
+   one buffer, with equal strides, do not overlap).
    Addresses are multiples of 16, strides of 8 elements. */
 VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* qkv, int qkv_type,
                              long long qkv_stride, int heads, const float* q_norm, const float* k_norm, float eps,
@@ -389,8 +390,8 @@ VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_bat
    f16; a bf16 q beyond +-65504 is taken as that), sums and softmax statistics in
    float.  A row that sees no position is zero; positions it does not see (later new
    tokens, rows of a page behind the length) may hold anything.  A row that sees an
-   infinite or NaN V of a later new token's position is NaN as a whole.  out must not
-   overlap q.  work: work_bytes of vc4_paged_attention_bytes for the same pages,
+   infinite or NaN V of a later new token's position is NaN as a whole.  An out
+   that overlaps q or the pool is refused, as a work that overlaps any of them.  work: work_bytes of vc4_paged_attention_bytes for the same pages,
    heads and batch bounds (NULL when that is 0), free again when the call's work is
    done. */
 VC4_API int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* q, int q_type,

@@ -659,3 +659,61 @@ def test_batches_off_their_elements_are_refused(name, off):
     _refused(lambda: _host_pages().append(batch, 64, "f32", 4, 64, "bf16"), "aligned to their elements")
     _refused(lambda: _host_pages().attend(batch, 64, "bf16", 4, 64, "bf16"), "aligned to their elements")
     _refused(lambda: _host_pages().attend_bytes(batch, 4), "aligned to their elements")
+
+
+# ---- buffers that overlap -----------------------------------------------------------------
+
+class _SomeGpu:
+    """A handle that a refusal does not look into."""
+    _h = 1
+
+
+@pytest.mark.parametrize("q,kw,words", [
+    (0x10000, {}, "q overlaps qkv"), (0x10000 + 4 * 512 * 4 - 16, {}, "q overlaps qkv"), (0x10000 - 16, {}, "q overlaps qkv"),
+    (0x10000 - 4 * 256 * 2 + 16, {}, "q overlaps qkv"),                       # the last row's end
+    (0x10000 + 512 * 4, dict(qkv_stride=600, q_stride=1200), None),            # in the rows' gaps: 88 floats < 256 bf16
+    (0x10000 + 512 * 4, dict(qkv_stride=1024, q_stride=2048), "pool"),         # fits the gaps
+    (0x10000 - 512, dict(qkv_stride=640, q_stride=1280), "pool"),              # ahead of each row
+    (0x10000 - 528, dict(qkv_stride=640, q_stride=1280), "q overlaps qkv"),    # and round into the row before
+    (0x10000 + 512 * 4, dict(qkv_stride=1024, q_stride=2040), "q overlaps qkv"),
+    (0x10000 + 4 * 512 * 4, {}, "pool"), (0x10000 - 4 * 256 * 2, {}, "pool")])
+def test_append_refuses_overlaps(q, kw, words):
+    """Rows of 512 f32 (4 + 2 * 2 heads of 64) and 256 bf16, four tokens; the pool lies over all."""
+    pages = _host_pages("q8", data=0x8000, pages=64)
+    pages.gpu = _SomeGpu()
+    _refused(lambda: pages.append(_host_batch(), 0x10000, "f32", 4, q, "bf16", **kw), words or "q overlaps qkv")
+
+
+@pytest.mark.parametrize("out,kw,words", [
+    (0x10000, {}, "out overlaps q"), (0x10000 + 2032, {}, "out overlaps q"), (0x10000 - 4080, {}, "out overlaps q"),
+    (0x10000 + 512, dict(q_stride=512, out_stride=256), "out overlaps q"),
+    (0x10000 + 512, dict(q_stride=768, out_stride=384), "out overlaps the pool"),
+    (0x10000 + 2048, {}, "out overlaps the pool"), (0x10000 - 4096, {}, "out overlaps the pool")])
+def test_attend_refuses_overlaps(out, kw, words):
+    """Rows of 256 bf16 and 256 f32, four tokens."""
+    pages = _host_pages("q8", data=0x8000, pages=64)
+    pages.gpu = _SomeGpu()
+    _refused(lambda: pages.attend(_host_batch(), 0x10000, "bf16", 4, out, "f32", **kw), words)
+
+
+@pytest.mark.gpu
+def test_rows_side_by_side_and_a_work_buffer_that_overlaps():
+    """q and out as columns of one buffer; the work buffer over q, out or the pool is refused."""
+    heads, dim, new = 4, 64, 90
+    gpu = vc4b200.GPU(0)
+    cache = Cache([3000], [new], "bf16", 16, 2, dim)
+    handle, batch = cache.handles(vc4b200, gpu)
+    need = handle.attend_bytes(batch, heads)
+    assert need > 0
+    both = torch.randn(new, 2 * heads * dim, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    q, out = both[:, : heads * dim], both[:, heads * dim:]
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    kw = dict(q_stride=both.stride(0), out_stride=both.stride(0))
+    for at in (q, out, cache.pool):
+        _refused(lambda: handle.attend(batch, q.data_ptr(), "bf16", heads, out.data_ptr(), "bf16", at.data_ptr(), need, **kw), "overlaps")
+    torch.cuda.synchronize()
+    handle.attend(batch, q.data_ptr(), "bf16", heads, out.data_ptr(), "bf16", work.data_ptr(), need, **kw)
+    gpu.sync()
+    want, mass, top = attention(cache, q, heads)
+    bound = attention_bound("bf16", "bf16", want, mass, top, dim)
+    assert int(cache.status) == 0 and bool(((out.double().reshape(want.shape) - want).abs() <= bound).all())

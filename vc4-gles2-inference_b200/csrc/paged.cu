@@ -403,6 +403,28 @@ std::string bad_rows(const char* what, const void* ptr, long long stride, long l
     return "";
 }
 
+// Rows of bytes, `stride` apart, and whether two sets of them share a byte.  Rows that lie
+// side by side in one buffer (equal strides) do not; of sets with different strides the
+// whole extents count.
+struct Extent {
+    const void* at;
+    size_t rows, stride, width;
+};
+bool meet(Extent a, Extent b) {
+    if (!a.rows || !b.rows) return false;
+    if ((uintptr_t)b.at < (uintptr_t)a.at) std::swap(a, b);
+    const size_t ahead = (uintptr_t)b.at - (uintptr_t)a.at;
+    if (ahead >= (a.rows - 1) * a.stride + a.width) return false;
+    if (a.rows == 1 || (b.rows > 1 && b.stride != a.stride)) return true;
+    const size_t in = ahead % a.stride;      // where b's rows start in a's
+    return in < a.width || a.stride - in < b.width;
+}
+size_t bytes_of(int type) { return type == VC4_F32 ? 4 : 2; }
+Extent pool_of(const vc4_pages* p) {
+    const size_t rows = (size_t)p->pages * 2 * p->kv_heads * p->page_len;
+    return {p->data, 1, 0, rows * p->head_dim * (p->format == VC4_KV_Q8 ? 1 : 2)};
+}
+
 int shift_of(int page_len) { return page_len == 16 ? 4 : page_len == 32 ? 5 : page_len == 64 ? 6 : page_len == 128 ? 7 : 8; }
 
 PagedArgs paged_args(const vc4_pages* p, const vc4_paged_batch* b) {
@@ -508,6 +530,10 @@ extern "C" int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_
     if (cos && (!aligned16(cos) || !aligned16(sin) || rope_len <= 0))
         return refuse("the rotation tables need rows, their addresses multiples of 16");
     if (!g) return refuse("gpu is null");
+    const Extent from{qkv, (size_t)b->tokens, qkv_stride * bytes_of(qkv_type), width * bytes_of(qkv_type)};
+    const Extent to{q, (size_t)b->tokens, q_stride * bytes_of(q_type), qw * bytes_of(q_type)};
+    if (meet(from, to)) return refuse("q overlaps qkv");
+    if (meet(from, pool_of(p)) || meet(to, pool_of(p))) return refuse("the pool overlaps qkv or q");
     if (!b->tokens || !b->max_new) return VC4_OK;
     OnDevice on(gpu_device(g));
     if (on.err != cudaSuccess) return fail(VC4_ECUDA, cudaGetErrorString(on.err));
@@ -570,11 +596,17 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
     if (!(scale2 >= FLT_MIN) || !(scale2 < INFINITY)) return refuse("scale's product with the pages' grid leaves float's range");
     if ((long long)b->tokens * heads > 0x7fffffffLL) return refuse("too many rows in one call");
     if (!g) return refuse("gpu is null");
+    const Extent from{q, (size_t)b->tokens, q_stride * bytes_of(q_type), width * bytes_of(q_type)};
+    const Extent to{out, (size_t)b->tokens, out_stride * bytes_of(out_type), width * bytes_of(out_type)};
+    if (meet(from, to)) return refuse("out overlaps q");
+    if (meet(to, pool_of(p))) return refuse("out overlaps the pool");
     int sms = 0;
     if (int e = sms_of(gpu_device(g), &sms)) return e;
     const AttnPlan pl = attn_plan(p, b, heads, sms, out_type);
     if (work_bytes < pl.bytes || (pl.bytes && (!work || !aligned16(work))))
         return refuse("the work buffer needs " + std::to_string(pl.bytes) + " bytes at a multiple of 16");
+    const Extent parts{work, pl.bytes ? 1u : 0u, 0, pl.bytes};
+    if (meet(parts, from) || meet(parts, to) || meet(parts, pool_of(p))) return refuse("the work buffer overlaps q, out or the pool");
     if (!b->tokens || !b->max_new) return VC4_OK;
     if ((long long)b->seqs * p->kv_heads * pl.row_tiles * pl.splits > 0x7fffffffLL) return refuse("too many rows in one call");
     OnDevice on(gpu_device(g));
