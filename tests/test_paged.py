@@ -717,3 +717,30 @@ def test_rows_side_by_side_and_a_work_buffer_that_overlaps():
     want, mass, top = attention(cache, q, heads)
     bound = attention_bound("bf16", "bf16", want, mass, top, dim)
     assert int(cache.status) == 0 and bool(((out.double().reshape(want.shape) - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["q8", "q16", "bf16", "f16"])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("length", [-1, -2 ** 31 + 1, -2 ** 31])
+def test_negative_lengths_see_nothing(fmt, new, length):
+    """However far below 0 a length lies: nothing is appended, the rows are zero, the others stand."""
+    cache = Cache([50 + new, 70 + new], [new, new], fmt, 16, 1, 64)
+    _check_attend(cache, 2, _kind(fmt), _kind(fmt))
+    cache.len[0] = length
+    before = cache.pool.clone()
+    t, kw = _append_case(cache, 2, "f32", "f32", False, True)
+    gpu = vc4b200.GPU(0)
+    handle, batch = cache.handles(vc4b200, gpu)
+    torch.cuda.synchronize()
+    handle.append(batch, t["qkv"].data_ptr(), "f32", 2, t["q"].data_ptr(), "f32", **kw)
+    gpu.sync()
+    mine = torch.from_numpy(cache.host_table[0][cache.host_table[0] >= 0].astype(np.int64)).cuda()
+    assert int(cache.status) == EINVAL and torch.equal(cache.pool[mine], before[mine]) and bool((t["q"][:new] == 7).all())
+    cache.status.zero_()
+    q = torch.randn(2 * new, 128, generator=torch.Generator().manual_seed(2)).to(TORCH[_kind(fmt)]).cuda()
+    out, _ = _attend(cache, 2, _kind(fmt), _kind(fmt), q)
+    want, mass, top = attention(cache, q, 2)
+    bound = attention_bound(fmt, _kind(fmt), want, mass, top, 64)
+    assert int(cache.status) == EINVAL and bool((out[:new] == 0).all())
+    assert bool(((out[new:].double().view_as(want[new:]) - want[new:]).abs() <= bound[new:]).all())

@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
         long long row = 0;
         if (tok >= c0 && tok < c1) {                 // rows behind the last sequence: none of this
             const int page_len = 1 << p.page_shift;
-            pos = p.len[s] - (c1 - tok);
+            pos = max(p.len[s], 0) - (c1 - tok);
             bool bad = pos < 0 || pos >= (long long)p.table_stride * page_len || (a.cos && pos >= a.rope_len) ||
                        c1 - c0 > p.max_new || c0 < 0 || c1 > p.tokens;
             if (!bad) {
