@@ -744,3 +744,20 @@ def test_negative_lengths_see_nothing(fmt, new, length):
     bound = attention_bound(fmt, _kind(fmt), want, mass, top, 64)
     assert int(cache.status) == EINVAL and bool((out[:new] == 0).all())
     assert bool(((out[new:].double().view_as(want[new:]) - want[new:]).abs() <= bound[new:]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv", [(4, 4), (64, 1)])
+@pytest.mark.parametrize("new,max_new", [(1, 1000), (3, 2 ** 31 - 1), (100, 2 ** 31 - 1)])
+def test_attend_bounds_far_above_the_tokens(heads, kv, new, max_new):
+    """max_new is a bound: one beyond the batch's rows asks for no more work than they are."""
+    cache = Cache([500 + new] * 40, [new] * 40, "q8", 16, kv, 64)
+    gpu = vc4b200.GPU(0)
+    (handle, tight), (_, wide) = cache.handles(vc4b200, gpu, max_new=40 * new), cache.handles(vc4b200, gpu, max_new=max_new)
+    assert handle.attend_bytes(tight, heads) == handle.attend_bytes(wide, heads)
+    _check_attend(cache, heads, "bf16", "bf16", max_new=max_new)
+    assert int(cache.status) == 0
+
+
+def test_bytes_of_too_many_rows_are_refused():
+    _refused(lambda: _host_pages().attend_bytes(_host_batch(tokens=2 ** 29, max_new=2 ** 29), 4), "too many rows")

@@ -467,7 +467,8 @@ struct AttnPlan {
 // work buffer, for a second kernel.
 AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int sms, int out_type) {
     AttnPlan pl{};
-    const long long rows = (long long)b->max_new * (heads / p->kv_heads);
+    // (a sequence has no more new tokens than the batch, whatever max_new allows)
+    const long long rows = (long long)std::min(b->max_new, b->tokens) * (heads / p->kv_heads);
     const bool many = rows > 64 || (rows > 32 && p->head_dim > 96 && (long long)b->seqs * p->kv_heads >= sms);
     pl.chunk = many && !(p->format == VC4_KV_Q16 && out_type != VC4_BF16);
     pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
@@ -564,6 +565,7 @@ extern "C" int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const v
     if (!m.empty()) return refuse(m);
     if (heads <= 0 || heads % p->kv_heads) return refuse("heads must be a positive multiple of kv_heads");
     if (!bytes) return refuse("bytes is null");
+    if ((long long)b->tokens * heads > 0x7fffffffLL) return refuse("too many rows in one call");
     if (!g) return refuse("gpu is null");
     int sms = 0;
     if (int e = sms_of(gpu_device(g), &sms)) return e;
