@@ -322,7 +322,8 @@ VC4_API int vc4_read_buffer(vc4_session* s, int slot, int buf, int n, float* out
    page id outside the pool, a position outside the page table or the rotation
    tables, a length below the new tokens, offsets that run backwards or past the
    batch's rows, a token id outside the vocabulary give VC4_EINVAL, a NaN logit or a row of logits without a finite value VC4_ERANGE; a
-   kernel's bounded wait that ran out VC4_ECUDA (the call's outputs are void). */
+   kernel's bounded wait that ran out VC4_ECUDA (the call's outputs are void, the rows it
+   was for NaN). */
 
 /* Element types of activations.  VC4_Q16I: int32 values on the q16 grid (1/256),
    the form of this engine's own logits. */

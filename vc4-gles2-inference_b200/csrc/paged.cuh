@@ -110,6 +110,14 @@ __device__ __forceinline__ void st_shared16(unsigned addr, const uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// For a block in which a bounded wait gave up, all its threads: the copies and products it
+// still has in flight end before its shared memory is used again or given back.
+__device__ __forceinline__ void wait_for_copies() {
+    const unsigned long long began = global_ns();
+    while (global_ns() - began < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+}
+
 template <int FMT> struct PagedBytes { static constexpr int v = FMT == P_Q8 ? 1 : 2; };
 
 // Two 16-bit operands in one register.
