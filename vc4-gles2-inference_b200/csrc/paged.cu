@@ -105,7 +105,7 @@ __device__ __forceinline__ void store_cache4(uint8_t* row, int i, float4 v) {
 // 1/sqrt(ss/hd + eps), w*(r*x), the rotation's products and sums rounded one by one, the
 // codec's floor(x*grid + 1/2).  (Packed products round like single ones.)
 template <int TIN, int FMT, int LPV>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, TIN == VC4_F32 ? 2 : 3) k_paged_append(AppendArgs a) {
     constexpr int N = kAppendVecs, NG = 32 / LPV;   // groups of a warp
     const PagedArgs& p = a.p;
     const int hd = p.head_dim, half = hd / 2, nvec = a.heads + 2 * p.kv_heads, turned = a.heads + p.kv_heads;
@@ -133,21 +133,16 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
     const int first = warp * NG + lane / LPV;
     fetch(first);
 
-    // offsets that start below 0, run backwards or end past the rows, wherever a token's look-up
-    // does not meet them: a sequence a thread
-    if (p.status)
-        for (long long i = (long long)blockIdx.x * kAppendThreads + threadIdx.x; i < p.seqs; i += (long long)gridDim.x * kAppendThreads)
-            if (p.cu[i] < 0 || p.cu[i + 1] < p.cu[i] || p.cu[i + 1] > p.tokens) paged_flag(p.status, VC4_EINVAL);
     if (warp < ntok) {
         const int tok = tok0 + warp, s = paged_find(p.cu, p.seqs, tok);
         const int c0 = p.cu[s], c1 = p.cu[s + 1];
         int pos = -1;
         long long row = 0;
-        if (tok >= c0 && tok < c1) {                 // rows behind the last sequence: none of this
+        if (tok >= c0 && tok < c1 && c0 >= 0 && c1 <= p.tokens) {   // rows of no sequence, or of a bad one: none of this
             const int page_len = 1 << p.page_shift;
             pos = max(p.len[s], 0) - (c1 - tok);
             bool bad = pos < 0 || pos >= (long long)p.table_stride * page_len || (a.cos && pos >= a.rope_len) ||
-                       c1 - c0 > p.max_new || c0 < 0 || c1 > p.tokens;
+                       c1 - c0 > p.max_new;
             if (!bad) {
                 const int page = p.table[(size_t)s * p.table_stride + (pos >> p.page_shift)];
                 bad = page < 0 || page >= p.pages;
@@ -163,6 +158,11 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
             s_row[warp] = row;
         }
     }
+    // offsets that start below 0, run backwards or end past the rows: a sequence a lane of the
+    // last warp, so that those no token's look-up meets are found too
+    if (warp == kAppendThreads / 32 - 1)
+        for (long long i = (long long)blockIdx.x * 32 + lane; i < p.seqs; i += (long long)gridDim.x * 32)
+            if (p.cu[i] < 0 || p.cu[i + 1] < p.cu[i] || p.cu[i + 1] > p.tokens) paged_flag(p.status, VC4_EINVAL);
     __syncthreads();
 
     const int es = FMT == P_Q8 ? 1 : 2;
