@@ -390,8 +390,8 @@ VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_bat
    VC4_BF16, VC4_F16.  Products run on the tensor cores (bf16 pages: bf16, others:
    f16; a bf16 q beyond +-65504 is taken as that), sums and softmax statistics in
    float.  A row that sees no position is zero; positions it does not see (later new
-   tokens, rows of a page behind the length) may hold anything.  A row that sees an
-   infinite or NaN V of a later new token's position is NaN as a whole.  An out
+   tokens, rows of a page behind the length) may hold anything.  An
+   infinite or NaN V makes its columns of the rows that see it infinite or NaN.  An out
    that overlaps q or the pool is refused, as a work that overlaps any of them.  work: work_bytes of vc4_paged_attention_bytes for the same pages,
    heads and batch bounds (NULL when that is 0), free again when the call's work is
    done. */

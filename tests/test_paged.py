@@ -761,3 +761,37 @@ def test_attend_bounds_far_above_the_tokens(heads, kv, new, max_new):
 
 def test_bytes_of_too_many_rows_are_refused():
     _refused(lambda: _host_pages().attend_bytes(_host_batch(tokens=2 ** 29, max_new=2 ** 29), 4), "too many rows")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim,new,past", [
+    (2, 1, 64, 5, 40), (8, 2, 128, 9, 300), (4, 4, 96, 7, 5000), (4, 1, 128, 100, 60), (2, 2, 64, 300, 200), (8, 1, 80, 90, 3000),
+    (4, 1, 48, 100, 60), (2, 1, 32, 200, 3000), (8, 2, 16, 70, 129), (1, 1, 16, 64, 0), (2, 2, 128, 513, 1000)])
+@pytest.mark.parametrize("out_kind", ["f32", "bf16"])
+def test_attend_wild_values_stay_in_their_columns(fmt, heads, kv, dim, new, past, out_kind):
+    """Infinite and NaN V of new tokens: their columns of the rows that see them are what the
+    sum is, infinite or NaN, every other value as without them, however many tokens are fed together."""
+    first, second = new // 3, new * 2 // 3
+    cache = Cache([33, past + new], [1, new], fmt, 16, kv, dim)
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(new + 1, heads * dim, generator=g).to(TORCH[fmt]).cuda()
+    clean, _ = _attend(cache, heads, fmt, out_kind, q)
+    inf, nan = float("inf"), float("nan")
+    plants = [(first, 0, inf), (second, 0, -inf), (second, dim - 1, nan), (first, dim // 2 + 1, -inf), (second, dim // 2 + 1, -inf)]
+    want = clean.view(new + 1, heads, dim).clone()
+    for at, d, value in plants:
+        pg, off = int(cache.host_table[1, (past + at) // 16]), (past + at) % 16
+        cache.pool[pg, 1, kv - 1, off, d] = value
+        want[1 + at:, heads - heads // kv:, d] = value
+    want[1 + second:, heads - heads // kv:, 0] = nan             # both infinities
+    out, _ = _attend(cache, heads, fmt, out_kind, q)
+    assert torch.equal(torch.nan_to_num(out, nan=7.5).view_as(want), torch.nan_to_num(want, nan=7.5))
+    for at in (first, second, new - 1):                          # the same row fed alone
+        one = Cache([past + at + 1], [1], fmt, 16, kv, dim)
+        one.pool, one.pages = cache.pool, cache.pages
+        one.table.copy_(cache.table[1:, : one.width])
+        alone, _ = _attend(one, heads, fmt, out_kind, q[1 + at: 2 + at])
+        a, b = alone.view(heads, dim), want[1 + at]
+        assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b))
+        assert torch.equal(a[torch.isinf(a)], b[torch.isinf(b)])

@@ -325,6 +325,13 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
     // max_new were not computed: leave them
     const int s = paged_find(p.cu, p.seqs, tok), c0 = p.cu[s];
     if (c0 < 0 || tok < c0 || tok >= p.cu[s + 1] || tok - c0 >= p.max_new) return;
+    bool wild = false;      // infinite or NaN values were taken out of this row
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        wild |= marked_wild(e[k].y);
+        e[k].y = fabsf(e[k].y);
+    }
+    wild = __any_sync(0xffffffffu, wild);
     float m = fmaxf(e[0].x, e[1].x);
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float w[2], l = 0.0f;
@@ -360,9 +367,19 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
             v.w = __fmaf_rn(wi[k], x[k].w, v.w);
         }
     }
-    if (d < hd)
-        store4_as(a.out, a.out_type, (long long)tok * a.out_stride + (long long)head * hd + d,
-                  make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+    if (d < hd) {
+        float y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        if (wild) {
+            const int r = (tok - c0) * a.group + head % a.group, r0 = r / kPagedChunkRows * kPagedChunkRows;
+            for (int k = 0; k < 4; k += 2) {
+                const float2 x = a.fmt == P_BF16 ? wild_sum<P_BF16>(p, s, head / a.group, a.group, r0, r, d + k)
+                                                 : wild_sum<P_F16>(p, s, head / a.group, a.group, r0, r, d + k);
+                y[k] += x.x;
+                y[k + 1] += x.y;
+            }
+        }
+        store4_as(a.out, a.out_type, (long long)tok * a.out_stride + (long long)head * hd + d, make_float4(y[0], y[1], y[2], y[3]));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -472,7 +489,7 @@ AttnPlan attn_plan(const vc4_pages* p, const vc4_paged_batch* b, int heads, int 
     const bool many = rows > 64 || (rows > 32 && p->head_dim > 96 && (long long)b->seqs * p->kv_heads >= sms);
     pl.chunk = many && !(p->format == VC4_KV_Q16 && out_type != VC4_BF16);
     pl.wr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const int per = pl.chunk ? 256 : 16 * pl.wr, tile = pl.chunk ? 128 : 64;
+    const int per = pl.chunk ? kPagedChunkRows : 16 * pl.wr, tile = pl.chunk ? 128 : 64;
     pl.row_tiles = (int)((rows + per - 1) / per);
     const long long units = (long long)b->seqs * p->kv_heads * std::max(1, pl.row_tiles);
     const int tiles = (b->max_len + tile - 1) / tile;
@@ -618,6 +635,7 @@ extern "C" int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_pag
     a.p = paged_args(p, b);
     a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.q_type = q_type; a.out_type = out_type;
     a.heads = heads; a.group = heads / p->kv_heads; a.row_tiles = pl.row_tiles; a.splits = pl.splits;
+    a.fmt = pfmt(p->format);
     a.scale2 = scale2;
     a.vscale = (float)grid;
     if (pl.bytes) {

@@ -32,6 +32,7 @@ struct PagedAttnArgs {
     void* out;
     long long q_stride, out_stride;
     int q_type, out_type, heads, group;
+    int fmt;                 // PFmt of the pages
     int row_tiles, splits;   // grid: ((sequence * kv_heads + head) * row_tiles + tile) * splits + split
     float scale2;            // score scale x log2 e x the K grid
     float vscale;            // the V grid
@@ -53,6 +54,7 @@ bool launch_paged_chunk_f16(const PagedAttnArgs& a, cudaStream_t st);
 namespace {
 
 constexpr int kPagedMaxSplits = 64;    // of the many-row kernel
+constexpr int kPagedChunkRows = 256;   // rows of its blocks
 constexpr int kPagedMaxCluster = 8;    // splits of the few-row kernel: blocks of a cluster
 
 __device__ __forceinline__ void paged_flag(int* status, int code) {
@@ -101,6 +103,54 @@ __device__ __forceinline__ uint4 tamed(uint4 v) {
     };
     return make_uint4(tame(v.x), tame(v.y), tame(v.z), tame(v.w));
 }
+// What the taken-out infinite and NaN V add to two values from column d of row r of sequence
+// s (rows of a block that starts at row r0): those of the positions the row sees and some
+// row of its block does not, read again from their pages; 0 where there are none.
+template <int FMT>
+__device__ __forceinline__ float2 wild_sum(const PagedArgs& p, int s, int kvh, int group, int r0, int r, int d) {
+    const int n = min(p.cu[s + 1], p.tokens) - p.cu[s], len = max(p.len[s], 0);
+    const int end = min(min(len, p.table_stride << p.page_shift), len - n + r / group + 1);
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+    for (int pos = max(0, len - n + r0 / group + 1); pos < end; ++pos) {
+        const int id = p.table[(size_t)s * p.table_stride + (pos >> p.page_shift)];
+        if (id < 0 || id >= p.pages) continue;
+        const size_t row = ((((size_t)id * 2 + 1) * p.kv_heads + kvh) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+        const unsigned w = *reinterpret_cast<const unsigned*>(reinterpret_cast<const unsigned short*>(p.data) + row * p.head_dim + d);
+        float2 x;
+        if (FMT == P_BF16) x = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+        else x = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        if (!(fabsf(x.x) < INFINITY)) sum.x += x.x;
+        if (!(fabsf(x.y) < INFINITY)) sum.y += x.y;
+    }
+    return sum;
+}
+// Adds them to the finished rows r0 .. r0 + count - 1, all threads of a block together.
+template <int FMT>
+__device__ __forceinline__ void add_wild(const PagedAttnArgs& a, int s, int kvh, int r0, int count) {
+    const int half = a.p.head_dim / 2;
+    for (int e = threadIdx.x; e < count * half; e += blockDim.x) {
+        const int r = r0 + e / half, d = e % half * 2;
+        const float2 w = wild_sum<FMT>(a.p, s, kvh, a.group, r0, r, d);
+        const long long i = (long long)(a.p.cu[s] + r / a.group) * a.out_stride + (long long)(kvh * a.group + r % a.group) * a.p.head_dim + d;
+        auto add = [](auto* v, float x) {
+            if (x != 0.0f) *v = (float)*v + x;
+        };
+        if (a.out_type == VC4_F32) {
+            add(reinterpret_cast<float*>(a.out) + i, w.x);
+            add(reinterpret_cast<float*>(a.out) + i + 1, w.y);
+        } else if (a.out_type == VC4_BF16) {
+            add(reinterpret_cast<__nv_bfloat16*>(a.out) + i, w.x);
+            add(reinterpret_cast<__nv_bfloat16*>(a.out) + i + 1, w.y);
+        } else {
+            add(reinterpret_cast<__half*>(a.out) + i, w.x);
+            add(reinterpret_cast<__half*>(a.out) + i + 1, w.y);
+        }
+    }
+}
+// A sum of weights, negative where such values belong to its row.
+__device__ __forceinline__ float mark_wild(float l) { return __int_as_float(__float_as_int(l) | (int)0x80000000u); }
+__device__ __forceinline__ bool marked_wild(float l) { return __float_as_int(l) < 0; }
 __device__ __forceinline__ uint4 ld_shared16(unsigned addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
