@@ -795,3 +795,61 @@ def test_attend_wild_values_stay_in_their_columns(fmt, heads, kv, dim, new, past
         a, b = alone.view(heads, dim), want[1 + at]
         assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b))
         assert torch.equal(a[torch.isinf(a)], b[torch.isinf(b)])
+
+
+# ---- q16 levels whole ---------------------------------------------------------------------
+
+def _levels(cache, sel, pos, levels):
+    """Plants int16 levels ([kv][dim] or one number) of K (0) or V (1) at a position of sequence 0."""
+    x = torch.as_tensor(levels).expand(cache.kv, cache.dim).to(torch.int16).contiguous()
+    cache.pool[int(cache.host_table[0, pos // 16]), sel, :, pos % 16] = swap16(x).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 48, 64, 128])
+@pytest.mark.parametrize("heads", [2, 32, 64, 128, 300])
+@pytest.mark.parametrize("kind,out_kind", [("f16", "f32"), ("bf16", "f32"), ("f16", "f16")])
+def test_attend_q16_scores_use_all_bits_of_a_level(dim, heads, kind, out_kind):
+    """f16 and float outputs: two positions whose levels, 16391 and 16393, an f16 operand rounds
+    8 times as far apart.  The bound is the definition's for exact operands (twice the products)."""
+    cache = Cache([2], [1], "q16", 16, 2, dim)
+    for pos, k, v in ((0, 16391, 16384), (1, 16393, -16384)):
+        _levels(cache, 0, pos, k)
+        _levels(cache, 1, pos, v)
+    q = torch.full((1, heads * dim), 8.0, dtype=TORCH[kind], device="cuda")
+    out, _ = _attend(cache, heads, kind, out_kind, q)
+    want, mass, top = attention(cache, q, heads)
+    bound = attention_bound("f16", out_kind, want, mass, top, 2 * dim)
+    rounded = 8 * math.tanh(-8 * 8 / 2048 * math.sqrt(dim))     # 16384 and 16400
+    assert float((rounded - want).abs().min()) > 4 * float(bound.max())
+    assert bool(((out.double().view_as(want) - want).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [16, 64, 80, 128])
+@pytest.mark.parametrize("heads", [2, 32, 64, 128, 300])
+def test_attend_q16_values_use_all_bits_of_a_level(dim, heads):
+    """Float outputs of one position are its V: 2^-21 for the exponential and the quotient, a
+    128th of what an f16 operand drops of an odd level near 2^14 (7 of 16391)."""
+    cache = Cache([1], [1], "q16", 16, 2, dim)
+    g = torch.Generator().manual_seed(dim)
+    v = torch.randint(-32768, 32768, (2, dim), generator=g)
+    v[:, :6] = torch.tensor([16391, -16391, 32767, -32768, 1, -1])
+    _levels(cache, 1, 0, v)
+    out, _ = _attend(cache, heads, "f16", "f32", torch.zeros(1, heads * dim, dtype=torch.float16, device="cuda"))
+    want = (v.double() / 2048).repeat_interleave(heads // 2, 0).cuda()
+    assert bool(((out.double().view_as(want) - want).abs() <= 2.0 ** -21 * want.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["q8", "q16", "bf16", "f16"])
+@pytest.mark.parametrize("seqs,new,length", [(2, 100, 3000), (40, 200, 900), (2, 700, 900)])
+def test_attend_many_rows_same_bits_twice(fmt, seqs, new, length):
+    """Split positions or not, on one stream and another: the same inputs, the same bits."""
+    cache = Cache([length - 3 * s for s in range(seqs)], [new] * seqs, fmt, 32, 2, 64)
+    q = torch.randn(cache.rows, 8 * 64, generator=torch.Generator().manual_seed(1)).to(TORCH[_kind(fmt)]).cuda()
+    a, _ = _attend(cache, 8, _kind(fmt), _kind(fmt), q)
+    side = torch.cuda.Stream()
+    for stream in (0, side.cuda_stream, 0):
+        b, _ = _attend(cache, 8, _kind(fmt), _kind(fmt), q, stream=stream)
+        assert torch.equal(a, b)
