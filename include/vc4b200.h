@@ -388,13 +388,16 @@ VC4_API int vc4_paged_append(vc4_gpu* g, const vc4_pages* p, const vc4_paged_bat
    h / (heads / kv_heads).  scale 0: 1/sqrt(head_dim).  q_type is VC4_BF16 or
    VC4_F16 and, for bf16 and f16 pages, the pages' own; out_type any of VC4_F32,
    VC4_BF16, VC4_F16.  Products run on the tensor cores (bf16 pages: bf16, others:
-   f16; a bf16 q beyond +-65504 is taken as that), sums and softmax statistics in
-   float.  A row that sees no position is zero; positions it does not see (later new
-   tokens, rows of a page behind the length) may hold anything.  An
+   f16), sums and softmax statistics in float; a softmax weight is rounded to the
+   operand type for its product with V.  Over q8 and q16 pages a bf16 q is taken as f16:
+   beyond +-65504 as that, below 2^-14 off by up to 2^-25.  A q16 level has 16 bits: with
+   a bf16 out it is rounded to f16's 11, with an f16 or float out all of them count.
+   A row that sees no position, or only scores of -inf, is zero; positions it does not
+   see (later new tokens, rows of a page behind the length) may hold anything.  An
    infinite or NaN V makes its columns of the rows that see it infinite or NaN.  An out
-   that overlaps q or the pool is refused, as a work that overlaps any of them.  work: work_bytes of vc4_paged_attention_bytes for the same pages,
-   heads and batch bounds (NULL when that is 0), free again when the call's work is
-   done. */
+   that overlaps q or the pool is refused, as is a work that overlaps any of them.  work:
+   work_bytes of vc4_paged_attention_bytes for the same pages, heads and batch bounds
+   (NULL when that is 0), free again when the call's work is done. */
 VC4_API int vc4_paged_attention(vc4_gpu* g, const vc4_pages* p, const vc4_paged_batch* b, const void* q, int q_type,
                                 long long q_stride, int heads, float scale, void* out, int out_type,
                                 long long out_stride, void* work, size_t work_bytes, void* stream);
@@ -409,15 +412,17 @@ VC4_API int vc4_paged_attention_bytes(vc4_gpu* g, const vc4_pages* p, const vc4_
    id, x) is accepted while u[row] * d(x) < p(x), d being the draft's row of
    draft_probs (one row for each draft of the batch in order, probs_stride apart; 0:
    vocab; sequences behind offsets that start below 0 or run backwards are skipped, for
-   their rows of it are unknown), or one at x and zero elsewhere when draft_probs is NULL.  The first
-   refused row is sampled from max(p - d, 0) normalised (from p where that is zero
-   everywhere), and the last row, when all are accepted, from p:
-   the first id whose cumulative sum exceeds u_sample[s] times the total, sums in
-   double.  next: per row the accepted draft, then the sampled id, then -1;
-   accepted (seqs): drafts accepted, 0 for a sequence without rows; prob (rows, or NULL): the target's probability
-   of each id in next, 0 where that is -1.  logits_type: VC4_F32, VC4_BF16, VC4_F16
-   or VC4_Q16I.  `rows` bounds cu[seqs].  NaN logits count as -inf.  An output that
-   overlaps an input or another output is refused. */
+   their rows of it are unknown), or one at x and zero elsewhere when draft_probs is
+   NULL.  The first refused row is sampled from max(p - d, 0) normalised (from p where
+   that is zero everywhere), and the last row, when all are accepted, from p: the first
+   id whose cumulative sum exceeds u_sample[s] times the total, sums in double.  next:
+   per row the accepted draft, then the sampled id, then -1; accepted (seqs): drafts
+   accepted, 0 for a sequence without rows; prob (rows, or NULL): the target's
+   probability of each id in next, 0 where that is -1.  logits_type: VC4_F32, VC4_BF16,
+   VC4_F16 or VC4_Q16I.  `rows` bounds cu[seqs]: logits, fed, u, next and prob have that
+   many rows, and all logits are read.  NaN logits count as -inf.  An output that overlaps
+   an input or another output is refused, as far as the host can tell: of draft_probs the
+   first rows - seqs rows are looked at, all it has where every sequence has a row. */
 VC4_API int vc4_verify_draft(vc4_gpu* g, int seqs, int rows, int vocab, const int* cu, const int* fed,
                              const void* logits, int logits_type, long long logits_stride, const float* draft_probs,
                              long long probs_stride, double temperature, const float* u, const float* u_sample,
