@@ -624,13 +624,13 @@ def test_append_flags_a_bad_offset_among_many_sequences():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("cu,good", [((0, 100, 201), [0, 1]), ((-1, 100, 200), [1]), ((0, 100, 1), [0]), ((100, 100, 200), [0, 1]),
-                                     ((-5, -1, 200), [])])
+@pytest.mark.parametrize("cu,good", [((0, 100, 201), [0]), ((-1, 100, 200), [1]), ((0, 100, 1), [0]), ((100, 100, 200), [0, 1]),
+                                     ((-5, -1, 200), []), ((0, 2 ** 31 - 1, 200), []), ((-2 ** 31, 100, 200), [1])])
 @pytest.mark.parametrize("heads,length", [(1, 300), (4, 3000), (8, 130)])
 def test_attend_leaves_rows_of_bad_offsets(heads, length, cu, good):
-    """Many rows, their positions split or not: a sequence that starts below 0 or ends before
-    it starts is skipped, its rows and those behind the batch stay; the others are the
-    definition's, one that runs past the rows with the rows there are."""
+    """Many rows, their positions split or not: a sequence that starts below 0, ends
+    before it starts or past the rows is skipped, its rows and those behind the batch stay;
+    the others are the definition's."""
     new, dim = 100, 64
     cache = Cache([length, length - 90], [new, new], "bf16", 16, 1, dim, rows=2 * new)
     # (a length below the new tokens is flagged too: 40 positions for 100 tokens)

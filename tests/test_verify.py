@@ -560,11 +560,11 @@ def test_verify_draft_rows_count_from_the_first_offset(first):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("cu,good,drafts", [([0, 3, 2], [0], 2), ([-1, 3, 6], [], 5), ([0, 3, 9], [0, 1], 4), ([4, 2, 6], [], 3),
-                                            ([0, 9, 3, 6], [0], 5), ([0, 2, 1, 4, 6], [0], 4)])
+@pytest.mark.parametrize("cu,good,drafts", [([0, 3, 2], [0], 2), ([-1, 3, 6], [], 5), ([0, 3, 9], [0], 2), ([4, 2, 6], [], 3),
+                                            ([0, 9, 3, 6], [], 5), ([0, 2, 1, 4, 6], [0], 4)])
 def test_verify_skips_draft_rows_behind_bad_offsets(cu, good, drafts):
-    """With draft probabilities: sequences behind offsets that start below 0 or run backwards
-    are flagged and skipped, those before them stand."""
+    """With draft probabilities: sequences behind offsets that start below 0 or run backwards,
+    and one that ends past the rows, are flagged and skipped, those before them stand."""
     rows, vocab = 6, 300
     lg, nxt, acc, status = _offsets(cu, rows, vocab, torch.ones(drafts, vocab, device="cuda"))
     assert status == EINVAL

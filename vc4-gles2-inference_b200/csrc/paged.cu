@@ -321,10 +321,10 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         e[k] = lane + 32 * k < a.splits ? a.ml[at + (lane + 32 * k) * step] : make_float2(-INFINITY, 0.0f);
-    // rows behind the last sequence, those of a sequence that starts below 0 and those beyond
-    // max_new were not computed: leave them
-    const int s = paged_find(p.cu, p.seqs, tok), c0 = p.cu[s];
-    if (c0 < 0 || tok < c0 || tok >= p.cu[s + 1] || tok - c0 >= p.max_new) return;
+    // rows of no sequence, of one whose offsets are bad and beyond max_new were not computed:
+    // leave them
+    const int s = paged_find(p.cu, p.seqs, tok), c0 = p.cu[s], c1 = p.cu[s + 1];
+    if (c0 < 0 || tok < c0 || tok >= c1 || c1 > p.tokens || tok - c0 >= p.max_new) return;
     bool wild = false;      // infinite or NaN values were taken out of this row
 #pragma unroll
     for (int k = 0; k < 2; ++k) {

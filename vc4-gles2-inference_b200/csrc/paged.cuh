@@ -108,7 +108,7 @@ __device__ __forceinline__ uint4 tamed(uint4 v) {
 // row of its block does not, read again from their pages; 0 where there are none.
 template <int FMT>
 __device__ __forceinline__ float2 wild_sum(const PagedArgs& p, int s, int kvh, int group, int r0, int r, int d) {
-    const int n = min(p.cu[s + 1], p.tokens) - p.cu[s], len = max(p.len[s], 0);
+    const int n = p.cu[s + 1] - p.cu[s], len = max(p.len[s], 0);
     const int end = min(min(len, p.table_stride << p.page_shift), len - n + r / group + 1);
     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
     __shared__ int s_first[W], s_ok[W], s_range;
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int s = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int c0 = a.cu[s], c1 = min(a.cu[s + 1], a.rows), n = c1 - c0, V = a.vocab;
+    const int c0 = a.cu[s], c1 = a.cu[s + 1], n = c1 - c0, V = a.vocab;
     s_tab[tid] = exp2((double)tid / 256);
     // this sequence's first row of draft_probs: a row for each of the batch before it, but
     // for the last row of every sequence that has any.  Behind offsets that start below 0 or
@@ -278,12 +278,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) k_verify_pick(VerifyArgs a)
     const bool writes = rank == 0;
     lost = __syncthreads_or(lost);
     pdl_wait();
-    if (c0 < 0 || n <= 0 || lost) {        // every block of the cluster leaves here
+    if (c0 < 0 || n <= 0 || c1 > a.rows || lost) {   // every block of the cluster leaves here
         if (tid == 0 && writes) a.accepted[s] = 0;
-        if (tid == 0 && (n || c0 < 0) && a.status) atomicMax(a.status, VC4_EINVAL);   // offsets that run backwards
+        if (tid == 0 && (n || c0 < 0 || c1 > a.rows) && a.status) atomicMax(a.status, VC4_EINVAL);   // bad offsets
         return;
     }
-    if (tid == 0 && a.cu[s + 1] > a.rows && a.status) atomicMax(a.status, VC4_EINVAL);
 
     // ---- the walk, W rows at a time, the same in every block ----
     int stop = n - 1, row_first = 0;
