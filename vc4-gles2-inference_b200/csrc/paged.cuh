@@ -125,11 +125,11 @@ __device__ __forceinline__ float2 wild_sum(const PagedArgs& p, int s, int kvh, i
     }
     return sum;
 }
-// Adds them to the finished rows r0 .. r0 + count - 1, all threads of a block together.
+// Adds them to the finished rows r0 .. r0 + count - 1: the first `threads` threads of a block.
 template <int FMT>
-__device__ __forceinline__ void add_wild(const PagedAttnArgs& a, int s, int kvh, int r0, int count) {
+__device__ __forceinline__ void add_wild(const PagedAttnArgs& a, int s, int kvh, int r0, int count, int threads) {
     const int half = a.p.head_dim / 2;
-    for (int e = threadIdx.x; e < count * half; e += blockDim.x) {
+    for (int e = threadIdx.x; e < count * half; e += threads) {
         const int r = r0 + e / half, d = e % half * 2;
         const float2 w = wild_sum<FMT>(a.p, s, kvh, a.group, r0, r, d);
         const long long i = (long long)(a.p.cu[s] + r / a.group) * a.out_stride + (long long)(kvh * a.group + r % a.group) * a.p.head_dim + d;
@@ -161,10 +161,13 @@ __device__ __forceinline__ void st_shared16(unsigned addr, const uint4 v) {
 }
 
 // For a block in which a bounded wait gave up, all its threads: the copies and products it
-// still has in flight end before its shared memory is used again or given back.
+// still has in flight end before its shared memory is used again or given back (warp 0
+// waits, the others for it).
 __device__ __forceinline__ void wait_for_copies() {
-    const unsigned long long began = global_ns();
-    while (global_ns() - began < 2000000ull) __nanosleep(1000);
+    if (threadIdx.x < 32) {
+        const unsigned long long began = global_ns();
+        while (global_ns() - began < 2000000ull) __nanosleep(1000);
+    }
     __syncthreads();
 }
 
