@@ -129,6 +129,7 @@ __device__ __forceinline__ float2 wild_sum(const PagedArgs& p, int s, int kvh, i
 template <int FMT>
 __device__ __forceinline__ void add_wild(const PagedAttnArgs& a, int s, int kvh, int r0, int count, int threads) {
     const int half = a.p.head_dim / 2;
+#pragma unroll 1
     for (int e = threadIdx.x; e < count * half; e += threads) {
         const int r = r0 + e / half, d = e % half * 2;
         const float2 w = wild_sum<FMT>(a.p, s, kvh, a.group, r0, r, d);
