@@ -2,8 +2,8 @@
 //
 // Two kernels.  The first reads every row once, a warp per chunk: the maximum, its first
 // place and sum exp((l - max)/T); it is bound by those bytes (256 sequences of 8 rows of
-// 73448 floats: 94 us, 6.4 TB/s).  The second, bound by its chain of joins and the double
-// operations of the sampled row (72 us there), takes a cluster of blocks per sequence: it
+// 73448 floats: 94 us, 6.4 TB/s).  The second (72 us there, no unit full: issue 43%, fp64
+// 26%; 1024 blocks in 1.7 waves) takes a cluster of blocks per sequence: it
 // joins the chunks, walks the drafts, and samples from the row that ends the walk.  A
 // sample depends on cumulative sums next to a border, so that row is summed in double, in
 // one pass: per warp's slice of ids S = sum e, and over the ids A whose e / S0 exceeds
