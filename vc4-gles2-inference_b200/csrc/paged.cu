@@ -467,7 +467,9 @@ struct AttnPlan {
 // few-row kernel, in blocks of the least of 16, 32 and 64 that holds them; more to
 // the many-row kernel, 256 a block; of large heads from 33 rows, where every SM has a
 // block (32 x 16 tokens over 4000 bf16 positions, 32/8 heads of 128: 133 us in blocks of
-// 64 rows, 111 in the many-row kernel; 61 x 5 over 2000, 16/2 of 64: 29 and 35).  q16
+// 64 rows, 111 in the many-row kernel; 61 x 5 over 2000, 16/2 of 64: 29 and 35; at 96 and 80
+// either may win, 32/8 heads, bf16, 32 x 16 over 4000 113 and 101, 104 and 98, 64 x 10 over
+// 1500 91 and 95, 85 and 93).  q16
 // pages with an f16 or float output stay with the few-row kernel, which holds a level in
 // two operands.
 // Splits of the few-row kernel: as many as the GPU holds at once, of three tiles of 64
